@@ -393,7 +393,7 @@ def _own(s):
     c = s["case"]
     op = c["op"]
     if op == "route":
-        h["routing"].top_k(h["logits"], SCORES[c["score"]], c["normalise"])
+        h["routing"].route(h["logits"], SCORES[c["score"]], c["normalise"])
         return h["result"]
     if op == "blocknorm":
         h["y"].block_norm(h["norm"], out=h["out"], out_norm=h["out_norm"])
@@ -408,7 +408,7 @@ def _own(s):
     if op == "grouped":
         r.linear(h["x"], h["w"], h["bias"], ACTS[c["act"]], out=h["out"])
         return s["out"]
-    r.top_k(h["logits"])
+    r.route(h["logits"])
     r.linear(h["x"], h["up"], None, ACTS[c["act"]], out=h["mid"])
     r.linear(h["mid"], h["down"], None, grouped_input=True, out=h["expert_out"])
     r.combine(h["expert_out"], h["norm"], out_norm=h["out"])
