@@ -339,9 +339,10 @@ def _fletcher():
 
 
 class _DeviceArray:
-    """Device memory of the framework, for torch.as_tensor."""
+    """Device memory of the framework, for torch.as_tensor; keeps its owner alive."""
 
-    def __init__(self, ptr, shape, kind):
+    def __init__(self, owner, ptr, shape, kind):
+        self.owner = owner
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": shape, "typestr": kind, "version": 3}
 
 
@@ -365,7 +366,7 @@ def _handles(s):
             r.assign(s["ids"].cpu().numpy(), s["weights"].cpu().numpy())
         if c["op"] == "route":
             p = r.device_pointers()
-            h["result"] = tuple(torch.as_tensor(_DeviceArray(p[n], shape, kind), device="cuda")
+            h["result"] = tuple(torch.as_tensor(_DeviceArray(r, p[n], shape, kind), device="cuda")
                                 for n, shape, kind in (("experts", (c["rows"], c["k"]), "<i4"),
                                                        ("weights", (c["rows"], c["k"]), "<f4"),
                                                        ("offsets", (c["experts"] + 1,), "<i4"),
