@@ -34,6 +34,7 @@ extern "C" {
 typedef void* CudaContextRef; /* cuda_bridge.h:14 */
 typedef void* CudaBufferRef;  /* cuda_bridge.h:15 */
 typedef void* CudaModelRef;
+typedef void* CudaRoutingRef;
 
 /* ---- status codes */
 enum {
@@ -127,6 +128,13 @@ int32_t Cuda_SetHalfConversion(CudaContextRef ctx, int32_t mode);
  * Memory comes from a stream-ordered pool and is zero-filled. */
 CudaBufferRef Cuda_Alloc(CudaContextRef ctx, int64_t size);
 CudaBufferRef Cuda_AllocTensor(CudaContextRef ctx, int64_t rows, int64_t cols, int32_t dtype);
+/* A buffer over device memory that the caller owns (a host framework's tensor): rows*cols dense
+ * elements of dtype at `ptr`, which must be memory of the context's device, aligned to the element
+ * size, and outlive the buffer; Cuda_FreeBuffer releases the handle alone.  The caller orders its
+ * own streams with the context's (Cuda_GetStream, Cuda_Synchronize).  As the contents can change
+ * behind this ABI, Cuda_Linear_Fused lays such a weight out anew in every call.  NULL on error.
+ * (No counterpart in the reference.) */
+CudaBufferRef Cuda_WrapTensor(CudaContextRef ctx, void* ptr, int64_t rows, int64_t cols, int32_t dtype);
 /* cuda_bridge.h:26 */
 int32_t Cuda_FreeBuffer(CudaContextRef ctx, CudaBufferRef buf);
 /* cuda_bridge.h:27-29: raw byte copies (synchronous with respect to the host). */
@@ -238,6 +246,95 @@ int32_t Cuda_ApplyRoPE_VarLen(CudaContextRef ctx, CudaBufferRef data, const int3
  * (No counterpart in the reference; the spec's pooling head.) */
 int32_t Cuda_MeanPoolL2(CudaContextRef ctx, CudaBufferRef hidden, const int32_t* lengths,
                         int32_t numSeqs, int64_t cols, CudaBufferRef out);
+
+/* ================================================================ expert feed-forward block
+ * The feed-forward block of an encoder whose rows are each sent to a few of many experts: a router
+ * chooses, products grouped by expert compute, a weighted sum joins, and the norms around the
+ * block follow.  (The reference has the dense block only.)  Shared rules:
+ *   - all calls enqueue on the context's stream, read sizes that depend on the routing on the
+ *     device alone, allocate nothing and never wait for the GPU, so that a sequence of them can be
+ *     captured into a CUDA graph (except Cuda_Routing_Assign, which reads host arrays);
+ *   - buffers are dense and row-major, and share one dtype except where noted;
+ *   - an output may not overlap an input unless its entry below says so.
+ *
+ * A routing holds, for up to max_rows rows and top_k choices a row: the experts chosen, their
+ * weights, and the order of the choices by expert.  Choice j of row r is pair r*top_k + j; pairs
+ * sorted by expert, then by pair, are given the slots 0, 1, ...; expert e owns the slots
+ * [offsets[e], offsets[e+1]).  A choice of -1 has no slot.  1 <= num_experts <= 256,
+ * 1 <= top_k <= min(16, num_experts), max_rows * top_k < 2^31.
+ * A routing's device memory belongs to its context (as a buffer's does): free it before the
+ * context.  The next Cuda_Routing_TopK or Assign overwrites it in stream order; graphs that share
+ * one routing must not run at the same time. */
+int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_experts, int32_t top_k,
+                            CudaRoutingRef* out);
+int32_t Cuda_Routing_Free(CudaRoutingRef routing);
+
+enum { FLETCHER_SCORE_SOFTMAX = 0, FLETCHER_SCORE_SIGMOID = 1 };
+/* Routes `rows` rows by their logits [rows, num_experts] (any dtype).  Each row's choices are its
+ * top_k largest logits in descending order, equal ones by the lower expert; -inf and NaN are never
+ * chosen, and a row with fewer than top_k others gets -1 with weight 0 for the rest.  The weight of
+ * a choice is the softmax over the row's eligible logits (if some are +inf they share the weight equally)
+ * or the logit's sigmoid; with normalise != 0 the weights of a row are divided by
+ * their sum (all 0 if that is 0); then all are multiplied by `scale`.  Weights are f32. */
+int32_t Cuda_Routing_TopK(CudaRoutingRef routing, CudaBufferRef logits, int64_t rows, int32_t scoring,
+                          int32_t normalise, float scale);
+/* Routes rows by choices the caller made: host arrays experts [rows, top_k] in [-1, num_experts)
+ * (an expert may appear twice in a row) and weights [rows, top_k], or NULL for all 1.  The arrays
+ * may be reused on return. */
+int32_t Cuda_Routing_Assign(CudaRoutingRef routing, const int32_t* experts, const float* weights, int64_t rows);
+/* The last routing, copied to host arrays; any may be NULL.  experts, weights and slots hold
+ * rows*top_k entries (slots -1 where there is none), offsets num_experts+1.  Synchronous. */
+int32_t Cuda_Routing_Read(CudaRoutingRef routing, int32_t* experts, float* weights, int32_t* slots,
+                          int32_t* offsets);
+/* The same arrays' device addresses (constant over the routing's life); any may be NULL. */
+int32_t Cuda_Routing_DevicePointers(CudaRoutingRef routing, void** experts, void** weights, void** slots,
+                                    void** offsets);
+
+/* Order of Cuda_Linear_Grouped's input rows: one row a token, gathered for each of its choices, or
+ * one row a slot. */
+enum { FLETCHER_ROWS_TOKENS = 0, FLETCHER_ROWS_SLOTS = 1 };
+/* Cuda_Linear_Fused for every expert at once: for each slot s of expert e,
+ *   result[s] = act(input[row of s] . weight[e] + bias[e]),
+ * weight [num_experts * inCols, outCols] (each expert's (in, out) matrix below the one before),
+ * bias [num_experts, outCols] or NULL, result [slots, outCols], or outCols/2 columns for SwiGLU
+ * (silu(first half) * second half).  act: IDENTITY, GELU, TANH or SWIGLU.  Sums are fp32.  `result`
+ * must hold rows*top_k rows; those behind the last slot are left as they were.  inCols and outCols
+ * are at most 2^24.  16-bit products whose inCols and output width are multiples of 8 and whose
+ * buffers are 16-byte aligned run on the tensor cores, straight from the (in, out) weights;
+ * others (and f32) on the fp32 units. */
+int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t inputOrder, int64_t inCols,
+                            CudaBufferRef weight, int64_t outCols, CudaBufferRef bias, CudaBufferRef result,
+                            int32_t activation);
+
+enum { FLETCHER_NORM_NONE = 0, FLETCHER_NORM_LAYER = 1, FLETCHER_NORM_RMS = 2 };
+/* What happens to a block's output y, row by row, in fp32 and rounded once per output:
+ *   u = residual_scale * residual + branch_scale * gate * post(y)      the residual stream
+ *   h = pre(u)                                                        the next block's input
+ * post and pre: none, LayerNorm ((x - mean) / sqrt(var + eps) * gamma + beta, as Cuda_LayerNorm)
+ * or RMS (x / sqrt(mean(x^2) + eps) * gamma).  gamma and beta are f32 [cols]; NULL means 1 and 0;
+ * RMS takes no beta.  residual [rows, cols] may be NULL (0).  gate may be NULL (1), or hold
+ * gate_rows = 1 row for all or gate_rows = rows. */
+typedef struct FletcherBlockNorm {
+  int32_t post_kind, pre_kind; /* FLETCHER_NORM_* */
+  float eps;
+  float residual_scale;
+  float branch_scale;
+  int32_t reserved; /* 0 */
+  int64_t gate_rows;
+  CudaBufferRef residual, gate;
+  CudaBufferRef post_gamma, post_beta, pre_gamma, pre_beta;
+} FletcherBlockNorm;
+/* u and h of y [rows, cols].  outResidual (u) may be NULL; outNorm (h) is given if and only if
+ * pre_kind is not NONE.  Each output may be the same buffer as y, as the residual or as a gate of
+ * `rows` rows.  cols <= 49152. */
+int32_t Cuda_BlockNorm(CudaContextRef ctx, CudaBufferRef y, int64_t rows, int64_t cols,
+                       const FletcherBlockNorm* norm, CudaBufferRef outResidual, CudaBufferRef outNorm);
+/* Joins the experts' outputs (grouped [slots, cols], as Cuda_Linear_Grouped wrote them):
+ *   y[r] = sum over the row's choices that have a slot, in order, of weight * grouped[slot]
+ * in fp32, followed by Cuda_BlockNorm's u and h of y; norm NULL means u = y.  An output may be the
+ * same buffer as the residual or as a gate of `rows` rows, not as `grouped`. */
+int32_t Cuda_Combine_Grouped(CudaRoutingRef routing, CudaBufferRef grouped, int64_t cols,
+                             const FletcherBlockNorm* norm, CudaBufferRef outResidual, CudaBufferRef outNorm);
 
 /* ================================================================ whole model
  * BertModel (bert.go:77-169) on the device, with fused kernels: tcgen05 GEMMs with fused

@@ -43,7 +43,7 @@ int32_t upload(Ctx* c, Temp& t, const void* h, int64_t bytes) {
 int32_t packed_weight(Ctx* c, Buf* w, int64_t K, int64_t N, bool swiglu, int bn, const void** out) {
   const int key = (swiglu ? 1 : 0) | (bn << 1);
   const int64_t bytes = K * N * 2;
-  if (!(w->packed && w->packed_key == key && w->packed_ver == w->version && w->packed_bytes == bytes)) {
+  if (!(!w->external && w->packed && w->packed_key == key && w->packed_ver == w->version && w->packed_bytes == bytes)) {
     dev_free(c, w->packed, w->packed_bytes);
     w->packed = nullptr;
     w->packed_bytes = 0;
@@ -64,7 +64,7 @@ int32_t packed_weight(Ctx* c, Buf* w, int64_t K, int64_t N, bool swiglu, int bn,
 // The bias widened to fp32 in the packed column order, cached like the weight.
 int32_t packed_bias(Ctx* c, Buf* b, int64_t N, bool swiglu, int bn, const float** out) {
   const int key = (swiglu ? 1 : 0) | (bn << 1);
-  if (!(b->bias32 && b->bias32_key == key && b->bias32_ver == b->version && b->bias32_bytes == N * 4)) {
+  if (!(!b->external && b->bias32 && b->bias32_key == key && b->bias32_ver == b->version && b->bias32_bytes == N * 4)) {
     dev_free(c, b->bias32, b->bias32_bytes);
     b->bias32 = nullptr;
     b->bias32_bytes = 0;

@@ -1,0 +1,417 @@
+// The norms around a block, its gate and residual (Cuda_BlockNorm), and the weighted sum of experts'
+// outputs in front of them (Cuda_Combine_Grouped): one pass over the rows, which stay in registers
+// in fp32 from the first load to the last store.
+//
+// Bound: HBM, at (inputs + outputs) * rows * cols * element size.  A row belongs to a team of 1 to 8
+// warps, whose lanes hold up to NV 16-byte vectors each; teams walk the rows with a stride.  Sums
+// are warp shuffles, joined through shared memory and a named barrier of the team where it has
+// several warps.  LayerNorm's variance is the mean of squared deviations (a second pass over
+// registers), as in Cuda_LayerNorm.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "routing.cuh"
+
+namespace fl {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxCols = 49152;  // the generic kernel keeps a row of fp32 in shared memory
+
+struct NormArgs {
+  const void* y;         // [rows, cols], or the slots' rows (combine)
+  const int32_t* slots;  // combine: [rows, top_k]
+  const float* weights;
+  int32_t top_k;
+  const void* residual;  // null: 0
+  const void* gate;      // null: 1
+  int64_t gate_step;     // elements from one row's gate to the next: 0 or cols
+  void* u;               // null: not stored
+  void* h;
+  const float *post_gamma, *post_beta, *pre_gamma, *pre_beta;
+  int32_t post, pre;
+  float eps, residual_scale, branch_scale;
+  int64_t rows;
+  int32_t cols;
+};
+
+template <typename T>
+union Pack {
+  uint4 q;
+  T t[16 / sizeof(T)];
+};
+
+// Sum over the team's lanes.  `red` has kSlots turns of 8 floats; turns alternate so that a warp
+// that is still reading one sum cannot meet the next sum's writes.
+constexpr int kTurns = 8;
+template <int WPR>
+__device__ __forceinline__ float team_sum(float s, float (*red)[8], int& turn) {
+  s = warp_sum(s);
+  if constexpr (WPR > 1) {
+    const int warp = threadIdx.x >> 5, team = warp / WPR;
+    if ((threadIdx.x & 31) == 0) red[turn][warp] = s;
+    asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(WPR * 32) : "memory");
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < WPR; i++) s += red[turn][team * WPR + i];
+    turn = (turn + 1) % kTurns;
+  }
+  return s;
+}
+
+// v = norm(v) for the team's row: lane t holds vectors t, t + TPR, ...; what lies past the row is 0
+// and stays out of the sums.
+template <int VEC, int NV, int WPR>
+__device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const float* __restrict__ gamma,
+                                         const float* __restrict__ beta, float eps, int t, int nvec, int cols,
+                                         float (*red)[8], int& turn) {
+  constexpr int TPR = 32 * WPR;
+  if (kind == FLETCHER_NORM_NONE) return;
+  float s = 0.f, mean = 0.f;
+  if (kind == FLETCHER_NORM_LAYER) {
+#pragma unroll
+    for (int i = 0; i < NV * VEC; i++) s += v[i];
+    mean = team_sum<WPR>(s, red, turn) / (float)cols;
+    s = 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    if (j * TPR + t < nvec) {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        v[j * VEC + i] -= mean;
+        s = fmaf(v[j * VEC + i], v[j * VEC + i], s);
+      }
+    }
+  }
+  const float inv = 1.0f / sqrtf(team_sum<WPR>(s, red, turn) / (float)cols + eps);
+#pragma unroll
+  for (int j = 0; j < NV; j++) {
+    const int at = j * TPR + t;
+    if (at < nvec) {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        float4 g = gamma ? __ldg(reinterpret_cast<const float4*>(gamma + at * VEC + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        float4 b = beta ? __ldg(reinterpret_cast<const float4*>(beta + at * VEC + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float* p = &v[j * VEC + i];
+        p[0] = fmaf(p[0] * inv, g.x, b.x);
+        p[1] = fmaf(p[1] * inv, g.y, b.y);
+        p[2] = fmaf(p[2] * inv, g.z, b.z);
+        p[3] = fmaf(p[3] * inv, g.w, b.w);
+      }
+    }
+  }
+}
+
+template <typename T, int NV, int WPR, bool COMBINE>
+__global__ void __launch_bounds__(kThreads) k_block_norm(const NormArgs a) {
+  constexpr int VEC = 16 / sizeof(T), TPR = 32 * WPR, TEAMS = kThreads / TPR;
+  __shared__ float red[kTurns][8];
+  int turn = 0;
+  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+  const int nvec = a.cols / VEC;
+  pdl_wait();
+  for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < a.rows; row += (int64_t)gridDim.x * TEAMS) {
+    float v[NV * VEC];
+    auto add = [&](const T* src, float scale, bool first) {
+      Pack<T> p[NV];
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (j * TPR + t < nvec) p[j].q = *reinterpret_cast<const uint4*>(src + (int64_t)(j * TPR + t) * VEC);
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          const float f = j * TPR + t < nvec ? to_f<T>(p[j].t[i]) : 0.f;
+          v[j * VEC + i] = first ? scale * f : fmaf(scale, f, v[j * VEC + i]);
+        }
+    };
+    if constexpr (COMBINE) {
+#pragma unroll
+      for (int i = 0; i < NV * VEC; i++) v[i] = 0.f;
+      for (int j = 0; j < a.top_k; j++) {
+        const int32_t slot = a.slots[row * a.top_k + j];
+        if (slot >= 0) add(reinterpret_cast<const T*>(a.y) + (int64_t)slot * a.cols, a.weights[row * a.top_k + j], false);
+      }
+    } else {
+      add(reinterpret_cast<const T*>(a.y) + row * a.cols, 1.0f, true);
+    }
+    norm_row<VEC, NV, WPR>(v, a.post, a.post_gamma, a.post_beta, a.eps, t, nvec, a.cols, red, turn);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      if (a.gate && j * TPR + t < nvec) {
+        Pack<T> g;
+        g.q = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_step +
+                                              (int64_t)(j * TPR + t) * VEC);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) v[j * VEC + i] *= to_f<T>(g.t[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; i++) v[j * VEC + i] *= a.branch_scale;
+    }
+    if (a.residual) add(reinterpret_cast<const T*>(a.residual) + row * a.cols, a.residual_scale, false);
+    auto store = [&](void* to) {
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        if (j * TPR + t < nvec) {
+          Pack<T> o;
+#pragma unroll
+          for (int i = 0; i < VEC; i++) o.t[i] = from_f<T>(v[j * VEC + i]);
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(to) + row * a.cols + (int64_t)(j * TPR + t) * VEC) = o.q;
+        }
+      }
+    };
+    if (a.u) store(a.u);
+    if (a.pre != FLETCHER_NORM_NONE) {
+      norm_row<VEC, NV, WPR>(v, a.pre, a.pre_gamma, a.pre_beta, a.eps, t, nvec, a.cols, red, turn);
+      store(a.h);
+    }
+  }
+}
+
+__device__ __forceinline__ float block_sum(float s, float* red) {
+  s = warp_sum(s);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; i++) s += red[i];
+  return s;
+}
+
+__device__ __forceinline__ void norm_generic(float* v, int kind, const float* gamma, const float* beta, float eps,
+                                             int cols, float* red) {
+  if (kind == FLETCHER_NORM_NONE) return;
+  float s = 0.f, mean = 0.f;
+  if (kind == FLETCHER_NORM_LAYER) {
+    for (int c = threadIdx.x; c < cols; c += kThreads) s += v[c];
+    mean = block_sum(s, red) / (float)cols;
+    s = 0.f;
+  }
+  for (int c = threadIdx.x; c < cols; c += kThreads) {
+    const float d = v[c] - mean;
+    v[c] = d;
+    s = fmaf(d, d, s);
+  }
+  const float inv = 1.0f / sqrtf(block_sum(s, red) / (float)cols + eps);
+  for (int c = threadIdx.x; c < cols; c += kThreads)
+    v[c] = fmaf(v[c] * inv, gamma ? gamma[c] : 1.0f, beta ? beta[c] : 0.0f);
+}
+
+// Any width and alignment: a block per row, the row in shared memory, each column always with the
+// same thread (so outputs may lie over inputs).
+template <typename T, bool COMBINE>
+__global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs a) {
+  extern __shared__ float v[];
+  __shared__ float red[kThreads / 32];
+  pdl_wait();
+  const T *y = reinterpret_cast<const T*>(a.y), *res = reinterpret_cast<const T*>(a.residual),
+          *gate = reinterpret_cast<const T*>(a.gate);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+      float s = 0.f;
+      if constexpr (COMBINE) {
+        for (int j = 0; j < a.top_k; j++) {
+          const int32_t slot = a.slots[row * a.top_k + j];
+          if (slot >= 0) s = fmaf(a.weights[row * a.top_k + j], to_f<T>(y[(int64_t)slot * a.cols + c]), s);
+        }
+      } else {
+        s = to_f<T>(y[row * a.cols + c]);
+      }
+      v[c] = s;
+    }
+    norm_generic(v, a.post, a.post_gamma, a.post_beta, a.eps, a.cols, red);
+    for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+      float s = v[c];
+      if (gate) s *= to_f<T>(gate[row * a.gate_step + c]);
+      s *= a.branch_scale;
+      if (res) s = fmaf(a.residual_scale, to_f<T>(res[row * a.cols + c]), s);
+      v[c] = s;
+      if (a.u) reinterpret_cast<T*>(a.u)[row * a.cols + c] = from_f<T>(s);
+    }
+    if (a.pre != FLETCHER_NORM_NONE) {
+      norm_generic(v, a.pre, a.pre_gamma, a.pre_beta, a.eps, a.cols, red);
+      for (int c = threadIdx.x; c < a.cols; c += kThreads) reinterpret_cast<T*>(a.h)[row * a.cols + c] = from_f<T>(v[c]);
+    }
+  }
+}
+
+template <typename T, int NV, int WPR, bool COMBINE>
+int32_t launch_vec(Ctx* c, const NormArgs& a) {
+  constexpr int TEAMS = kThreads / (32 * WPR);
+  const int64_t blocks = std::min<int64_t>((a.rows + TEAMS - 1) / TEAMS, (int64_t)c->num_sms * 8);
+  FL_CUDA(c, launch_pdl(k_block_norm<T, NV, WPR, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
+  FL_LAUNCH(c);
+  return FLETCHER_OK;
+}
+
+template <typename T, bool COMBINE>
+int32_t launch_norm(Ctx* c, const NormArgs& a) {
+  constexpr int VEC = 16 / sizeof(T);
+  const void* ptrs[] = {a.y, a.residual, a.gate, a.u, a.h, a.post_gamma, a.post_beta, a.pre_gamma, a.pre_beta};
+  bool vec = a.cols % VEC == 0;
+  for (const void* p : ptrs) vec = vec && ((uintptr_t)p & 15) == 0;
+  const int nvec = a.cols / VEC;
+  if (vec && nvec <= 1024) {
+    // The fewest warps a row whose lanes hold at most four vectors each.
+    if (nvec <= 32) return launch_vec<T, 1, 1, COMBINE>(c, a);
+    if (nvec <= 64) return launch_vec<T, 2, 1, COMBINE>(c, a);
+    if (nvec <= 96) return launch_vec<T, 3, 1, COMBINE>(c, a);
+    if (nvec <= 128) return launch_vec<T, 4, 1, COMBINE>(c, a);
+    if (nvec <= 192) return launch_vec<T, 3, 2, COMBINE>(c, a);
+    if (nvec <= 256) return launch_vec<T, 4, 2, COMBINE>(c, a);
+    if (nvec <= 384) return launch_vec<T, 3, 4, COMBINE>(c, a);
+    if (nvec <= 512) return launch_vec<T, 4, 4, COMBINE>(c, a);
+    if (nvec <= 768) return launch_vec<T, 3, 8, COMBINE>(c, a);
+    return launch_vec<T, 4, 8, COMBINE>(c, a);
+  }
+  auto kern = k_block_norm_generic<T, COMBINE>;
+  const int smem = a.cols * 4;
+  static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
+  if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
+    FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxCols * 4));
+    attr_set[c->device & 63].store(true, std::memory_order_release);
+  }
+  const int64_t blocks = std::min<int64_t>(a.rows, (int64_t)c->num_sms * 8);
+  FL_CUDA(c, launch_pdl(kern, dim3((unsigned)blocks), dim3(kThreads), smem, c->stream, a));
+  FL_LAUNCH(c);
+  return FLETCHER_OK;
+}
+
+template <bool COMBINE>
+int32_t launch_norm_dt(Ctx* c, int32_t dt, const NormArgs& a) {
+  if (dt == FLETCHER_BF16) return launch_norm<__nv_bfloat16, COMBINE>(c, a);
+  if (dt == FLETCHER_F16) return launch_norm<__half, COMBINE>(c, a);
+  return launch_norm<float, COMBINE>(c, a);
+}
+
+// Fills and checks what both entry points share.  `y` is [y_rows, cols]; in_place: outputs may be y.
+int32_t setup(Ctx* c, const char* op, const Buf* y, int64_t y_rows, bool in_place, int64_t rows, int64_t cols,
+              const FletcherBlockNorm* n, Buf* u, Buf* h, NormArgs* a) {
+  FL_CHECK(c, y, "%s: null buffer", op);
+  const int32_t dt = y->dtype;
+  FL_CHECK(c, cols >= 1 && cols <= kMaxCols, "%s: %lld columns outside [1, %d]", op, (long long)cols, kMaxCols);
+  FL_CHECK(c, rows >= 0 && rows <= INT32_MAX, "%s: %lld rows", op, (long long)rows);
+  FL_CHECK(c, holds(c, y, y_rows * cols), "%s: input must hold %lldx%lld on the context's device", op,
+           (long long)y_rows, (long long)cols);
+  const FletcherBlockNorm none{FLETCHER_NORM_NONE, FLETCHER_NORM_NONE, 0.f, 0.f, 1.f, 0, 0, nullptr, nullptr, nullptr,
+                               nullptr, nullptr, nullptr};
+  if (!n) n = &none;
+  FL_CHECK(c, n->post_kind >= FLETCHER_NORM_NONE && n->post_kind <= FLETCHER_NORM_RMS && n->pre_kind >= FLETCHER_NORM_NONE &&
+                  n->pre_kind <= FLETCHER_NORM_RMS,
+           "%s: unknown norm", op);
+  FL_CHECK(c, n->reserved == 0, "%s: the reserved field must be 0", op);
+  FL_CHECK(c, n->eps >= 0.f && std::isfinite(n->eps), "%s: eps must be finite and not negative", op);
+  FL_CHECK(c, u || h, "%s: no output", op);
+  FL_CHECK(c, (h != nullptr) == (n->pre_kind != FLETCHER_NORM_NONE),
+           "%s: the normed output is given exactly when there is a pre norm", op);
+  const int64_t total = rows * cols, es = dtype_size(dt), bytes = total * es;
+  const Buf *res = reinterpret_cast<const Buf*>(n->residual), *gate = reinterpret_cast<const Buf*>(n->gate);
+  FL_CHECK(c, !res || (res->dtype == dt && holds(c, res, total)), "%s: residual must be %lldx%lld of the input's dtype",
+           op, (long long)rows, (long long)cols);
+  FL_CHECK(c, !gate || n->gate_rows == 1 || n->gate_rows == rows, "%s: gate_rows must be 1 or the rows", op);
+  const bool wide_gate = gate && n->gate_rows == rows && rows != 1;
+  FL_CHECK(c, !gate || (gate->dtype == dt && holds(c, gate, (wide_gate ? rows : 1) * cols)),
+           "%s: gate must be %lldx%lld of the input's dtype", op, (long long)n->gate_rows, (long long)cols);
+  const struct {
+    CudaBufferRef ref;
+    const float** to;
+    int32_t kind;
+    bool shift;
+  } affine[] = {{n->post_gamma, &a->post_gamma, n->post_kind, false},
+                {n->post_beta, &a->post_beta, n->post_kind, true},
+                {n->pre_gamma, &a->pre_gamma, n->pre_kind, false},
+                {n->pre_beta, &a->pre_beta, n->pre_kind, true}};
+  Buf* outs[2] = {u, h};
+  for (Buf* o : outs) {
+    if (!o) continue;
+    FL_CHECK(c, o->dtype == dt && holds(c, o, total), "%s: outputs must be %lldx%lld of the input's dtype", op,
+             (long long)rows, (long long)cols);
+    // An output lies over an input either not at all or element for element.
+    FL_CHECK(c, (in_place && o->ptr == y->ptr) || !overlap(o->ptr, bytes, y->ptr, y_rows * cols * es),
+             "%s: an output overlaps the input", op);
+    FL_CHECK(c, !res || o->ptr == res->ptr || !overlap(o->ptr, bytes, res->ptr, bytes),
+             "%s: an output overlaps the residual", op);
+    FL_CHECK(c, !gate || (o->ptr == gate->ptr && n->gate_rows == rows) ||
+                    !overlap(o->ptr, bytes, gate->ptr, (wide_gate ? rows : 1) * cols * es),
+             "%s: an output overlaps the gate", op);
+  }
+  FL_CHECK(c, !u || !h || !overlap(u->ptr, bytes, h->ptr, bytes), "%s: the outputs overlap", op);
+  for (const auto& f : affine) {
+    const Buf* b = reinterpret_cast<const Buf*>(f.ref);
+    *f.to = nullptr;
+    if (!b) continue;
+    FL_CHECK(c, f.kind != FLETCHER_NORM_NONE, "%s: gamma or beta without its norm", op);
+    FL_CHECK(c, !(f.shift && f.kind == FLETCHER_NORM_RMS), "%s: the RMS norm takes no beta", op);
+    FL_CHECK(c, b->dtype == FLETCHER_F32 && holds(c, b, cols), "%s: gamma/beta must be f32 [%lld]", op, (long long)cols);
+    for (Buf* o : outs)
+      FL_CHECK(c, !o || !overlap(o->ptr, bytes, b->ptr, cols * 4), "%s: an output overlaps gamma or beta", op);
+    *f.to = (const float*)b->ptr;
+  }
+  a->y = y->ptr;
+  a->residual = res ? res->ptr : nullptr;
+  a->gate = gate ? gate->ptr : nullptr;
+  a->gate_step = wide_gate ? cols : 0;
+  a->u = u ? u->ptr : nullptr;
+  a->h = h ? h->ptr : nullptr;
+  a->post = n->post_kind;
+  a->pre = n->pre_kind;
+  a->eps = n->eps;
+  a->residual_scale = n->residual_scale;
+  a->branch_scale = n->branch_scale;
+  a->rows = rows;
+  a->cols = (int32_t)cols;
+  return FLETCHER_OK;
+}
+
+}  // namespace
+}  // namespace fl
+
+using namespace fl;
+
+extern "C" {
+
+int32_t Cuda_BlockNorm(CudaContextRef ctx, CudaBufferRef y, int64_t rows, int64_t cols, const FletcherBlockNorm* norm,
+                       CudaBufferRef outResidual, CudaBufferRef outNorm) {
+  Ctx* c = reinterpret_cast<Ctx*>(ctx);
+  if (!c) return FLETCHER_ERR_INVALID;
+  DeviceGuard g(c);
+  FL_CHECK(c, norm, "BlockNorm: null parameters");
+  const Buf* yb = reinterpret_cast<Buf*>(y);
+  Buf *u = reinterpret_cast<Buf*>(outResidual), *h = reinterpret_cast<Buf*>(outNorm);
+  NormArgs a{};
+  const int32_t rc = setup(c, "BlockNorm", yb, rows, true, rows, cols, norm, u, h, &a);
+  if (rc || rows == 0) return rc;
+  touch(u);
+  touch(h);
+  return launch_norm_dt<false>(c, yb->dtype, a);
+}
+
+int32_t Cuda_Combine_Grouped(CudaRoutingRef routing, CudaBufferRef grouped, int64_t cols, const FletcherBlockNorm* norm,
+                             CudaBufferRef outResidual, CudaBufferRef outNorm) {
+  Routing* r = as_routing(routing);
+  if (!r) return FLETCHER_ERR_INVALID;
+  Ctx* c = r->c;
+  DeviceGuard g(c);
+  FL_CHECK(c, r->device == c->device, "Combine_Grouped: the routing was made on another device");
+  FL_CHECK(c, r->rows >= 0, "Combine_Grouped: nothing routed yet");
+  const Buf* yb = reinterpret_cast<Buf*>(grouped);
+  Buf *u = reinterpret_cast<Buf*>(outResidual), *h = reinterpret_cast<Buf*>(outNorm);
+  NormArgs a{};
+  const int32_t rc = setup(c, "Combine_Grouped", yb, r->pairs(), false, r->rows, cols, norm, u, h, &a);
+  if (rc) return rc;
+  for (const Buf* o : {u, h})
+    FL_CHECK(c, !o || !overlap(o->ptr, r->rows * cols * dtype_size(yb->dtype), r->mem, r->bytes),
+             "Combine_Grouped: an output overlaps the routing");
+  if (r->rows == 0) return FLETCHER_OK;
+  touch(u);
+  touch(h);
+  a.slots = r->slots;
+  a.weights = r->weights;
+  a.top_k = r->top_k;
+  return launch_norm_dt<true>(c, yb->dtype, a);
+}
+
+}  // extern "C"

@@ -44,6 +44,8 @@ struct Buf {
   int64_t bytes = 0;
   int64_t rows = 0, cols = 0;
   int32_t dtype = FLETCHER_F32;
+  int device = 0;         // where the memory is
+  bool external = false;  // the caller's memory (Cuda_WrapTensor): never freed, nothing derived is kept
   // Write counter: bumped by every ABI call that may change the contents (see touch()).
   uint64_t version = 0;
   // Cuda_Linear_Fused's derived copies of a 16-bit weight / bias, valid while `version` equals

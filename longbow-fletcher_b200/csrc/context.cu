@@ -299,6 +299,7 @@ CudaBufferRef Cuda_AllocTensor(CudaContextRef ctx, int64_t rows, int64_t cols, i
   b->rows = rows;
   b->cols = cols;
   b->dtype = dtype;
+  b->device = c->device;
   b->bytes = rows * cols * dtype_size(dtype);
   if (dev_alloc(c, &b->ptr, b->bytes) != FLETCHER_OK) {
     delete b;
@@ -312,12 +313,45 @@ CudaBufferRef Cuda_Alloc(CudaContextRef ctx, int64_t size) {
   return Cuda_AllocTensor(ctx, 1, (size + 3) / 4, FLETCHER_F32);
 }
 
+CudaBufferRef Cuda_WrapTensor(CudaContextRef ctx, void* ptr, int64_t rows, int64_t cols, int32_t dtype) {
+  Ctx* c = C(ctx);
+  if (!c) return nullptr;
+  DeviceGuard g(c);
+  auto refuse = [&](const char* why) -> CudaBufferRef {
+    set_error(c, FLETCHER_ERR_INVALID, "WrapTensor: %s", why);
+    return nullptr;
+  };
+  if (dtype < 0 || dtype > 2) return refuse("unknown dtype");
+  const int64_t es = dtype_size(dtype);
+  if (rows < 0 || cols < 0 || (cols > 0 && rows > INT64_MAX / es / cols)) return refuse("bad shape");
+  if (rows * cols > 0) {
+    if ((uintptr_t)ptr % (uintptr_t)es != 0) return refuse("pointer not aligned to its element size");
+    cudaPointerAttributes at{};
+    if (!ptr || cudaPointerGetAttributes(&at, ptr) != cudaSuccess ||
+        (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)) {
+      cudaGetLastError();
+      return refuse("not device memory");
+    }
+    if (at.type == cudaMemoryTypeDevice && at.device != c->device) return refuse("memory of another device");
+  }
+  Buf* b = new Buf();
+  b->ctx = c;
+  b->ptr = ptr;
+  b->rows = rows;
+  b->cols = cols;
+  b->dtype = dtype;
+  b->device = c->device;
+  b->external = true;
+  b->bytes = rows * cols * es;
+  return b;
+}
+
 int32_t Cuda_FreeBuffer(CudaContextRef ctx, CudaBufferRef buf) {
   Buf* b = B(buf);
   if (!b) return FLETCHER_OK;
   Ctx* c = ctx ? C(ctx) : b->ctx;
   DeviceGuard g(c);
-  dev_free(c, b->ptr, b->bytes);
+  if (!b->external) dev_free(c, b->ptr, b->bytes);
   dev_free(c, b->packed, b->packed_bytes);
   dev_free(c, b->bias32, b->bias32_bytes);
   delete b;

@@ -1,0 +1,57 @@
+// The routing of rows to experts: what Cuda_Routing_* fill and the grouped products and the
+// combine read.
+#pragma once
+#include "kernels.cuh"
+
+namespace fl {
+
+constexpr int kMaxExperts = 256;
+constexpr int kMaxTopK = 16;
+
+struct Routing {
+  Ctx* c = nullptr;
+  int device = 0;
+  int64_t max_rows = 0;
+  int32_t num_experts = 0, top_k = 0;
+  int64_t rows = -1;  // rows of the last routing; -1: none yet
+  void* mem = nullptr;  // one allocation for the arrays below
+  int64_t bytes = 0;
+  int32_t* experts = nullptr;  // [pairs]
+  float* weights = nullptr;    // [pairs]
+  int32_t* slots = nullptr;    // [pairs] slot of each pair, -1: none
+  int32_t* pair_of = nullptr;  // [pairs] pair of each slot; behind the last slot unspecified
+  int32_t* offsets = nullptr;  // [num_experts + 1]
+  int32_t* hist = nullptr;     // [blocks, num_experts] choices of each expert in a block's rows
+  int64_t pairs() const { return rows * top_k; }
+};
+
+inline Routing* as_routing(CudaRoutingRef r) { return reinterpret_cast<Routing*>(r); }
+
+// Whether [a, a+na) and [b, b+nb) share memory.
+inline bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
+
+// A buffer of the context's device that holds `elems` elements.
+inline bool holds(const Ctx* c, const Buf* b, int64_t elems) {
+  return b && b->device == c->device && elems >= 0 && elems <= b->bytes / dtype_size(b->dtype);
+}
+
+// What a grouped product reads and writes (grouped_simt.cu, grouped_tc.cu).
+struct GroupedArgs {
+  const void* x;     // [tokens or slots, K]
+  const void* w;     // [experts * K, N]
+  const void* bias;  // [experts, N] or null
+  void* out;         // [slots, n_out]
+  int64_t K, N, n_out;
+  int64_t x_rows;          // rows of x
+  const int32_t* offsets;  // [experts + 1]
+  const int32_t* pair_of;  // rows of x are tokens: slot s reads row pair_of[s] / top_k; null: row s
+  int32_t top_k, experts;
+  int64_t pairs;  // upper bound of the slots
+  int32_t act;
+};
+int32_t launch_grouped_simt(Ctx* c, int32_t dtype, const GroupedArgs& a);
+
+}  // namespace fl

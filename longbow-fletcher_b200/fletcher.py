@@ -1,6 +1,8 @@
 """Python host binding of libcuda_fletcher.so (ctypes), mirroring the reference's Go device
 interface for the embedding forward pass.
 
+    Routing  : rows sent to experts (Cuda_Routing_*), their grouped products and the weighted sum;
+               no counterpart in the reference
     Backend  ~ device.Backend  (internal/device/device.go:137-162)
     Tensor   ~ device.Tensor   (internal/device/device.go:5-117), the methods the hot path uses
     BertModel~ model.BertModel (internal/embeddings/model/bert.go:77-169) on the device
@@ -26,6 +28,9 @@ F32, F16, BF16 = 0, 1, 2
 ACT_IDENTITY, ACT_GELU, ACT_TANH, ACT_SOFTMAX, ACT_SWIGLU = 0, 1, 2, 3, 4
 POOL_CLS_TANH, POOL_MEAN_L2 = 0, 1
 HALF_REFERENCE, HALF_RNE = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+ROWS_TOKENS, ROWS_SLOTS = 0, 1
+NORM_NONE, NORM_LAYER, NORM_RMS = 0, 1, 2
 DTYPES = {"f32": F32, "f16": F16, "bf16": BF16}
 _NP = {F32: np.float32, F16: np.float16}
 
@@ -53,6 +58,7 @@ def _sig(L):
         "Cuda_MemGetInfo": (i32, [vp, i64p, i64p]),
         "Cuda_Alloc": (vp, [vp, i64]),
         "Cuda_AllocTensor": (vp, [vp, i64, i64, i32]),
+        "Cuda_WrapTensor": (vp, [vp, vp, i64, i64, i32]),
         "Cuda_FreeBuffer": (i32, [vp, vp]),
         "Cuda_CopyToDevice": (i32, [vp, i64, vp, i64]),
         "Cuda_CopyToHost": (i32, [vp, i64, vp, i64]),
@@ -78,6 +84,15 @@ def _sig(L):
         "Cuda_ApplyRoPE": (i32, [vp, vp, i64, i64, i32, i32]),
         "Cuda_ApplyRoPE_VarLen": (i32, [vp, vp, i32p, i32, i32, i32, f32]),
         "Cuda_MeanPoolL2": (i32, [vp, vp, i32p, i32, i64, vp]),
+        "Cuda_Routing_Create": (i32, [vp, i64, i32, i32, ctypes.POINTER(vp)]),
+        "Cuda_Routing_Free": (i32, [vp]),
+        "Cuda_Routing_TopK": (i32, [vp, vp, i64, i32, i32, f32]),
+        "Cuda_Routing_Assign": (i32, [vp, i32p, f32p, i64]),
+        "Cuda_Routing_Read": (i32, [vp, i32p, f32p, i32p, i32p]),
+        "Cuda_Routing_DevicePointers": (i32, [vp] + 4 * [ctypes.POINTER(vp)]),
+        "Cuda_Linear_Grouped": (i32, [vp, vp, i32, i64, vp, i64, vp, vp, i32]),
+        "Cuda_BlockNorm": (i32, [vp, vp, i64, i64, vp, vp, vp]),
+        "Cuda_Combine_Grouped": (i32, [vp, vp, i64, vp, vp, vp]),
         "Cuda_Model_Create": (i32, [vp, vp, i32, ctypes.POINTER(vp)]),
         "Cuda_Model_LoadRaw": (i32, [vp, f32p, i64]),
         "Cuda_Model_WeightCount": (i64, [vp]),
@@ -200,6 +215,17 @@ class Backend:
     def new_tensor(self, r, c, data=None, dtype=None):
         return Tensor(self, r, c, self.dtype if dtype is None else dtype, data)
 
+    def wrap(self, ptr, r, c, dtype=None):
+        """A Tensor over (r, c) dense elements of device memory that the caller owns and keeps alive."""
+        dt = self.dtype if dtype is None else dtype
+        buf = lib().Cuda_WrapTensor(self.ctx, ctypes.c_void_p(ptr), r, c, dt)
+        if not buf:
+            self.check(1)  # FLETCHER_ERR_INVALID
+        return Tensor(self, r, c, dt, buf=buf)
+
+    def routing(self, max_rows, num_experts, top_k):
+        return Routing(self, max_rows, num_experts, top_k)
+
     def synchronize(self):
         self.check(lib().Cuda_Synchronize(self.ctx))
 
@@ -232,11 +258,11 @@ class Tensor:
     view sharing the buffer (cpu_backend.go:306-314); only Mul reads the flag, as in the
     reference, where every other op sees the stored layout."""
 
-    def __init__(self, be: Backend, r, c, dtype, data=None):
+    def __init__(self, be: Backend, r, c, dtype, data=None, buf=None):
         self.be, self.rows, self.cols, self.dtype = be, int(r), int(c), dtype
         self.trans = False
         self._owner = None
-        self.buf = lib().Cuda_AllocTensor(be.ctx, self.rows, self.cols, dtype)
+        self.buf = buf or lib().Cuda_AllocTensor(be.ctx, self.rows, self.cols, dtype)
         if not self.buf:
             be.check(3)
         if data is not None:
@@ -380,11 +406,124 @@ class Tensor:
         self.be.check(lib().Cuda_ApplyRoPE_VarLen(self.be.ctx, self.buf, _i32p(lens), lens.size, heads, head_dim,
                                                   base))
 
+    def block_norm(self, norm: "BlockNorm", out=None, out_norm=None):
+        """Cuda_BlockNorm of this block output: (u, h), the residual stream and its norm.  The outputs
+        may be given (this tensor and the residual among them); with neither, u is made, and h if
+        there is a pre norm.  A tensor that is neither given nor made is None."""
+        out, out_norm = norm._outputs(self, self.rows, out, out_norm)
+        self.be.check(lib().Cuda_BlockNorm(self.be.ctx, self.buf, self.rows, self.cols, norm._ref(self.rows),
+                                           out.buf if out else None, out_norm.buf if out_norm else None))
+        return out, out_norm
+
     def mean_pool_l2(self, lengths):
         lens = np.ascontiguousarray(lengths, np.int32)
         out = Tensor(self.be, lens.size, self.cols, F32)
         self.be.check(lib().Cuda_MeanPoolL2(self.be.ctx, self.buf, _i32p(lens), lens.size, self.cols, out.buf))
         return out
+
+
+class CBlockNorm(ctypes.Structure):
+    """Matches FletcherBlockNorm in include/fletcher_cuda.h."""
+    _fields_ = [("post_kind", ctypes.c_int32), ("pre_kind", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("residual_scale", ctypes.c_float), ("branch_scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("gate_rows", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in (
+                    "residual", "gate", "post_gamma", "post_beta", "pre_gamma", "pre_beta")]
+
+
+class BlockNorm:
+    """What happens to a block's output y (FletcherBlockNorm):
+    u = residual_scale * residual + branch_scale * gate * post(y), h = pre(u)."""
+
+    def __init__(self, post=NORM_NONE, pre=NORM_NONE, eps=1e-12, residual=None, gate=None, residual_scale=1.0,
+                 branch_scale=1.0, post_gamma=None, post_beta=None, pre_gamma=None, pre_beta=None):
+        self._tensors = dict(residual=residual, gate=gate, post_gamma=post_gamma, post_beta=post_beta,
+                             pre_gamma=pre_gamma, pre_beta=pre_beta)  # kept alive with the handles
+        self.c = CBlockNorm(post, pre, eps, residual_scale, branch_scale, 0, gate.rows if gate is not None else 0,
+                            **{k: t.buf for k, t in self._tensors.items() if t is not None})
+        self._p = ctypes.byref(self.c)
+
+    def _ref(self, rows):
+        for name, need in (("residual", rows), ("gate", self.c.gate_rows)):
+            t = self._tensors[name]
+            if t is not None and t.rows < need:
+                raise FletcherError(1, f"BlockNorm: {name} has {t.rows} rows, {need} are needed")
+        return self._p
+
+    def _outputs(self, y, rows, out, out_norm):
+        if out is None and out_norm is None:
+            out = Tensor(y.be, rows, y.cols, y.dtype)
+            if self.c.pre_kind != NORM_NONE:
+                out_norm = Tensor(y.be, rows, y.cols, y.dtype)
+        return out, out_norm
+
+
+class Routing:
+    """Rows sent to experts (Cuda_Routing_*): up to max_rows rows, top_k of num_experts each."""
+
+    def __init__(self, be: Backend, max_rows, num_experts, top_k):
+        self.be, self.num_experts, self.top_k, self.rows = be, num_experts, top_k, 0
+        h = ctypes.c_void_p()
+        self.h = None
+        be.check(lib().Cuda_Routing_Create(be.ctx, max_rows, num_experts, top_k, ctypes.byref(h)))
+        self.h = h
+
+    def __del__(self):
+        try:
+            if self.h and self.be.ctx:
+                lib().Cuda_Routing_Free(self.h)
+        except Exception:
+            pass
+
+    def route(self, logits: Tensor, scoring=SCORE_SOFTMAX, normalise=True, scale=1.0):
+        """Routes every row of logits (rows, num_experts) to its top_k largest."""
+        if logits.cols != self.num_experts:
+            raise FletcherError(1, f"Routing: logits have {logits.cols} columns for {self.num_experts} experts")
+        self.be.check(lib().Cuda_Routing_TopK(self.h, logits.buf, logits.rows, scoring, int(normalise), scale))
+        self.rows = logits.rows
+
+    def assign(self, experts, weights=None):
+        """Routes by given choices: host arrays (rows, top_k), -1 for none; weights default to 1."""
+        e = np.ascontiguousarray(experts, np.int32).reshape(-1, self.top_k)
+        w = None if weights is None else np.ascontiguousarray(weights, np.float32).reshape(-1, self.top_k)
+        if w is not None and w.shape != e.shape:
+            raise FletcherError(1, f"Routing: {w.shape} weights for {e.shape} choices")
+        self.be.check(lib().Cuda_Routing_Assign(self.h, _i32p(e), None if w is None else _f32p(w), e.shape[0]))
+        self.rows = e.shape[0]
+
+    def read(self):
+        """The last routing on the host: experts, weights, slots (rows, top_k) and offsets."""
+        shape = (self.rows, self.top_k)
+        e, s = np.empty(shape, np.int32), np.empty(shape, np.int32)
+        w, o = np.empty(shape, np.float32), np.empty(self.num_experts + 1, np.int32)
+        self.be.check(lib().Cuda_Routing_Read(self.h, _i32p(e), _f32p(w), _i32p(s), _i32p(o)))
+        return {"experts": e, "weights": w, "slots": s, "offsets": o}
+
+    def device_pointers(self):
+        p = [ctypes.c_void_p() for _ in range(4)]
+        self.be.check(lib().Cuda_Routing_DevicePointers(self.h, *(ctypes.byref(x) for x in p)))
+        return dict(zip(("experts", "weights", "slots", "offsets"), (x.value for x in p)))
+
+    def linear(self, x: Tensor, w: Tensor, b: "Tensor | None" = None, act=ACT_IDENTITY, grouped_input=False, out=None):
+        """Cuda_Linear_Grouped: w (num_experts * in, out), b (num_experts, out); one output row a slot.
+        x holds one row a token, or with grouped_input one row a slot."""
+        if w.rows != self.num_experts * x.cols:
+            raise FletcherError(1, f"Linear_Grouped: weight has {w.rows} rows, not {self.num_experts} x {x.cols}")
+        y = out or Tensor(self.be, self.rows * self.top_k, w.cols // 2 if act == ACT_SWIGLU else w.cols, x.dtype)
+        self.be.check(lib().Cuda_Linear_Grouped(self.h, x.buf, ROWS_SLOTS if grouped_input else ROWS_TOKENS, x.cols,
+                                                w.buf, w.cols, b.buf if b is not None else None, y.buf, act))
+        return y
+
+    def combine(self, grouped: Tensor, norm: "BlockNorm | None" = None, out=None, out_norm=None):
+        """Cuda_Combine_Grouped: the weighted sum of each row's slots, then the norm's u and h.
+        Without a norm returns the sum, else (u, h) as Tensor.block_norm does."""
+        if norm is None:
+            out = out or Tensor(self.be, self.rows, grouped.cols, grouped.dtype)
+            self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, None, out.buf, None))
+            return out
+        out, out_norm = norm._outputs(grouped, self.rows, out, out_norm)
+        self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, norm._ref(self.rows),
+                                                 out.buf if out else None, out_norm.buf if out_norm else None))
+        return out, out_norm
 
 
 class BertModel:
