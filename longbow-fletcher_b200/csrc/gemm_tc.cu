@@ -740,6 +740,23 @@ int32_t make_tma_map_2d(Ctx* c, CUtensorMap* m, int32_t dtype, const void* ptr, 
   return tc::make_map(c, m, dtype, ptr, rows, cols, ld, box_cols, box_rows);
 }
 
+// 3D map over dense [planes, rows, cols]: box {box_cols, box_rows, 1}; rows past a plane's end read
+// as zero, not as the next plane's.
+int32_t make_tma_map_3d(Ctx* c, CUtensorMap* m, int32_t dtype, const void* ptr, uint64_t planes, uint64_t rows,
+                        uint64_t cols, uint32_t box_cols, uint32_t box_rows) {
+  auto fn = tc::encode_fn();
+  if (!fn) return set_error(c, FLETCHER_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {cols, rows, planes};
+  cuuint64_t strides[2] = {cols * 2, rows * cols * 2};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(m, dtype == FLETCHER_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(c, FLETCHER_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FLETCHER_OK;
+}
+
 // FLETCHER_GEMM_PAIR=0 selects single-SM tiles everywhere (for A/B measurement).
 bool gemm_pair_enabled() {
   static const bool on = [] {

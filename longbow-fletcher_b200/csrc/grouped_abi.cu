@@ -61,6 +61,7 @@ int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t
   a.offsets = r->offsets;
   a.pair_of = inputOrder == FLETCHER_ROWS_TOKENS ? r->pair_of : nullptr;
   a.act = activation;
+  if (grouped_tc_supported(dt, a)) return launch_grouped_tc(c, dt, a);
   return launch_grouped_simt(c, dt, a);
 }
 

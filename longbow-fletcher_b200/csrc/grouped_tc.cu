@@ -1,0 +1,543 @@
+// Grouped products on tcgen05 / TMEM / TMA, bf16 and fp16: for every slot s of expert e,
+// out[s] = act(x[row(s)] . W[e] + b[e]), W [E][K, N] as the framework stores Linear weights,
+// (in, out).
+//
+// Layout: rows of x are K-major operands, fetched in 128-byte-swizzled 64-wide slabs: by TMA tiles
+// where a group's rows lie together, by TMA gathers of four rows where slots point at tokens.  W is
+// read as it is stored: its rows are K, its columns contiguous, so boxes of 64 K x 64 columns are
+// MN-major operands (64 columns = one 128-byte swizzle row, 8-row K groups 1024 bytes apart, column
+// blocks 8 KB apart).  No weight is packed or copied, and SwiGLU's gate and up columns are simply
+// fetched from the two halves of a row into one tile.  Rows of K past the end read as zero on both
+// sides (x by its width, W by its own dimension, so one expert's rows never meet the next one's).
+//
+// The number of rows of each group is known on the device only.  Every CTA reads the offsets,
+// computes how many row tiles each group has, and walks the same list of (row tile, column tile)
+// pairs with a stride; tiles never span groups, so the last tile of a group computes rows it does
+// not store.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "routing.cuh"
+#include "tc_common.cuh"
+
+namespace fl {
+
+int32_t make_tma_map_2d(Ctx* c, CUtensorMap* m, int32_t dtype, const void* ptr, uint64_t rows, uint64_t cols,
+                        uint64_t ld, uint32_t box_cols, uint32_t box_rows);
+int32_t make_tma_map_3d(Ctx* c, CUtensorMap* m, int32_t dtype, const void* ptr, uint64_t planes, uint64_t rows,
+                        uint64_t cols, uint32_t box_cols, uint32_t box_rows);
+
+namespace tcg {
+
+using namespace tc;
+
+constexpr int BM = 128, BK = 64;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr int kBox = 32 * 128;  // an epilogue warp's output box: 32 rows x 64 columns x 2 bytes
+constexpr int kColBlock = 64 * BK * 2;  // 64 columns of W x 64 rows of K
+
+// BN: accumulator columns of a tile.  PAIR: the tile is 256 rows, computed by two CTAs (two SMs) with
+// cta_group::2; each loads its 128 rows of x and half of the columns of W.
+template <int BN, bool PAIR>
+struct Cfg {
+  static constexpr int TILE_M = PAIR ? 2 * BM : BM;
+  static constexpr int B_COLS = PAIR ? BN / 2 : BN;  // columns of W loaded by one CTA
+  static constexpr int A_BYTES = BM * BK * 2;
+  static constexpr int B_BYTES = B_COLS * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int OUT_BYTES = kEpiWarps * kBox;
+  static constexpr int TABLE_BYTES = (kMaxExperts + 1 + 32) * 4;
+  static constexpr int TAIL_BYTES = 384 + TABLE_BYTES;  // barriers, then the groups' table
+  static constexpr int STAGES_FIT = (232448 - 1024 - TAIL_BYTES - OUT_BYTES) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_FIT < 8 ? STAGES_FIT : 8;
+  static constexpr int OUT_OFF = STAGES * STAGE_BYTES;
+  static constexpr int BAR_OFF = OUT_OFF + OUT_BYTES;
+  static constexpr int TABLE_OFF = BAR_OFF + 384;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int SMEM = BAR_OFF + TAIL_BYTES + 1024 /*alignment slack*/;
+  static_assert((2 * STAGES + 8) * 8 <= 384, "barrier area");
+  static_assert(SMEM <= 232448, "shared memory budget");
+};
+
+struct Args {
+  const int32_t* offsets;
+  const int32_t* pair_of;
+  const void* bias;
+  void* out;
+  int32_t* err;
+  int64_t N, n_out;
+  int32_t E, top_k, num_kb, n_tiles, act;
+};
+
+// Four rows of a 2-D tensor by index (64 columns from x), one below the other.
+template <bool PAIR>
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int x, const int (&r)[4]) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+        : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// MN-major operand of several 64-column blocks: 128-byte swizzle, K groups of 8 rows 1024 bytes
+// apart (SBO), column blocks kColBlock apart (LBO).
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(kColBlock >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+// The groups' row tiles: prefix[e] tiles come before group e's.  Filled by the whole block.
+__device__ __forceinline__ void fill_table(const int32_t* offsets, int E, int tile_m, int32_t* prefix, int32_t* tmp) {
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  int n = 0;
+  if (t < E) n = (offsets[t + 1] - offsets[t] + tile_m - 1) / tile_m;
+  int s = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 31) tmp[warp] = s;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < warp; w++) before += tmp[w];
+  if (t < E) prefix[t + 1] = before + s;
+  if (t == 0) prefix[0] = 0;
+  __syncthreads();
+}
+
+struct Tile {
+  int e, first, end, nb;  // expert, first slot, end of its group, column tile
+};
+// Tiles are asked for in ascending order.
+struct Walk {
+  const int32_t *offsets, *prefix;
+  int n_tiles, tile_m, e = -1, first = 0, end = 0;
+  __device__ __forceinline__ Tile at(int tile) {
+    const int mt = tile / n_tiles;
+    if (e < 0 || prefix[e + 1] <= mt) {
+      do e++;
+      while (prefix[e + 1] <= mt);
+      first = offsets[e];
+      end = offsets[e + 1];
+    }
+    return {e, first + (mt - prefix[e]) * tile_m, end, tile - mt * n_tiles};
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void add_bias32(float (&v)[32], const T* b, int64_t col, int64_t cols) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    if (col + i < cols) {
+      union {
+        uint4 q;
+        T t[8];
+      } u;
+      u.q = __ldg(reinterpret_cast<const uint4*>(b + col + i));
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[i + j] += to_f<T>(u.t[j]);
+    }
+  }
+}
+
+__device__ __forceinline__ float silu16(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+
+// Row-per-lane 64 values -> 16-byte chunks of T.
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
+// Persistent: warp 0 loads (TMA tiles or gathers), warp 1 issues the MMAs and owns the TMEM, warps 2-9
+// drain one accumulator while the next tile fills the other.  As the dense GEMM: bounded waits, and
+// on expiry every role leaves after what it issued has landed.
+template <typename T, int BN, bool PAIR, bool GATED, bool GATHER>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_grouped_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const __grid_constant__ CUtensorMap tmC, const Args args) {
+  using C = Cfg<BN, PAIR>;
+  constexpr int OUT_N = GATED ? BN / 2 : BN;  // output columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::STAGES * C::A_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem + C::TABLE_OFF);
+  int32_t* tmp = prefix + kMaxExperts + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = PAIR ? cluster_ctarank() : 0;
+  const int first_tile = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+  const int tile_stride = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], kEpiWarps * (PAIR ? 2 : 1));
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmC) : "memory");
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(C::TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                   "r"(C::TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  pdl_wait();  // the routing and x are the previous kernels' work
+  fill_table(args.offsets, args.E, C::TILE_M, prefix, tmp);
+  tc_fence_before();
+  if constexpr (PAIR)
+    cluster_sync();  // both CTAs' barriers are initialised before any cross-CTA signal
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const int num_tiles = prefix[args.E] * args.n_tiles;
+  Walk walk{args.offsets, prefix, args.n_tiles, C::TILE_M};
+
+  if (warp == 0) {
+    // Producer: lane 0 loads tiles; in a gather every lane fetches its own four rows.
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, issued_par = 0;
+    int rows[4] = {}, next[4] = {};
+    auto fetch = [&](const Tile& t, int (&r)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int s = t.first + (int)crank * BM + 4 * lane + i;
+        r[i] = args.pair_of[s < t.end ? s : t.first];  // rows past the group are computed, not stored
+      }
+    };
+    Tile cur{};
+    if (first_tile < num_tiles) {
+      cur = walk.at(first_tile);
+      if constexpr (GATHER) fetch(cur, next);
+    }
+    bool ok = true;
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
+      const Tile t = cur;
+      if constexpr (GATHER) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) rows[i] = next[i] / args.top_k;
+      }
+      if (tile + tile_stride < num_tiles) {  // the next tile's rows are on their way during this one
+        cur = walk.at(tile + tile_stride);
+        if constexpr (GATHER) fetch(cur, next);
+      }
+      const int a_row = t.first + (int)crank * BM;
+      for (int kb = 0; kb < args.num_kb; kb++) {
+        ok = GATHER || lane == 0 ? mbar_wait_spin(&empty[stage], phase ^ 1, abort, args.err) : true;
+        if constexpr (GATHER) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* a = sA + stage * C::A_BYTES;
+        uint8_t* b = sB + stage * C::B_BYTES;
+        // In a pair both CTAs' loads complete on the even CTA's barrier, which expects both.
+        const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
+        if (lane == 0) {
+          if (crank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * C::STAGE_BYTES);
+          if constexpr (!GATHER) {
+            if constexpr (PAIR)
+              tma_load_2d_pair(a, &tmA, fb, kb * BK, a_row);
+            else
+              tma_load_2d(a, &tmA, &full[stage], kb * BK, a_row);
+          }
+#pragma unroll
+          for (int i = 0; i < C::B_COLS / 64; i++) {
+            const int col = i * 64 + (int)crank * C::B_COLS;  // accumulator column
+            const int x = GATED ? t.nb * OUT_N + col % OUT_N + (col >= OUT_N ? (int)args.n_out : 0) : t.nb * BN + col;
+            tma_load_3d<PAIR>(b + i * kColBlock, &tmB, fb, x, kb * BK, t.e);
+          }
+        }
+        if constexpr (GATHER) tma_gather4<PAIR>(a + lane * 512, &tmA, fb, kb * BK, rows);
+        issued |= 1u << stage;
+        issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    // Leaving early: the loads in flight land before the CTA exits (in a pair they complete on the even
+    // CTA's barriers; the odd CTA cannot pass the last cluster barrier before that one has seen them).
+    if (lane == 0 && *abort && crank == 0)
+      for (int s = 0; s < C::STAGES; s++)
+        if ((issued >> s) & 1) mbar_drain(&full[s], (issued_par >> s) & 1);
+  } else if (warp == 1) {
+    if (lane == 0 && crank == 0) {
+      const uint32_t id = idesc<T, C::TILE_M, BN, true>();
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride, ++it) {
+        const int acc = it & 1;
+        if (!mbar_wait_spin(&tempty[acc], ((it >> 1) & 1) ^ 1, abort, args.err)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * BN;
+        for (int kb = 0; kb < args.num_kb; kb++) {
+          if (!(ok = mbar_wait_spin(&full[stage], phase, abort, args.err))) break;
+          tc_fence_after();
+          const uint64_t da = sw128_desc(smem_u32(sA + stage * C::A_BYTES));
+          const uint64_t db = desc_mn(smem_u32(sB + stage * C::B_BYTES));
+#pragma unroll
+          for (int k = 0; k < BK / 16; k++) {  // K += 16: 32 bytes along x's rows, 16 rows (2 KB) down W's blocks
+            if constexpr (PAIR)
+              mma_f16_pair(d, da + 2 * k, db + (uint64_t)k * (2048 >> 4), id, (kb | k) != 0);
+            else
+              mma_f16(d, da + 2 * k, db + (uint64_t)k * (2048 >> 4), id, (kb | k) != 0);
+          }
+          if constexpr (PAIR)
+            mma_commit_pair(&empty[stage]);
+          else
+            mma_commit(&empty[stage]);
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        if constexpr (PAIR)
+          mma_commit_pair(&tfull[acc]);
+        else
+          mma_commit(&tfull[acc]);
+      }
+      if (*abort) {  // the MMAs issued so far complete before TMEM is freed
+        if constexpr (PAIR)
+          mma_commit_pair(drain);
+        else
+          mma_commit(drain);
+        mbar_drain(drain, 0);
+      }
+    }
+  } else {
+    // Epilogue: warps 2-5 take the first half of a tile's output columns, warps 6-9 the second; warp w
+    // reads TMEM lanes 32 * (w % 4) .., its lanes' rows.
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    constexpr int UNITS = OUT_N / 128;  // 64-column units of a warp
+    static_assert(UNITS >= 1, "tile width");
+    uint8_t* box = smem + C::OUT_OFF + (warp - 2) * kBox;
+    const uint32_t tempty_lead = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0;
+    T* out = reinterpret_cast<T*>(args.out);
+    int it = 0;
+    for (int tile = first_tile; tile < num_tiles; tile += tile_stride, ++it) {
+      const Tile t = walk.at(tile);
+      const int acc = it & 1;
+      const int row0 = t.first + (int)crank * BM + q * 32;
+      const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN;
+      const T* bias = args.bias ? reinterpret_cast<const T*>(args.bias) + (int64_t)t.e * args.N : nullptr;
+      if (!mbar_wait_spin(&tfull[acc], (it >> 1) & 1, abort, args.err)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int u = 0; u < UNITS; u++) {
+        const int c0 = half * (OUT_N / 2) + u * 64;  // first output column of the unit within the tile
+        const int64_t ocol = (int64_t)t.nb * OUT_N + c0;
+        float v[64];
+        float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
+        float (&hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
+        if constexpr (GATED) {
+#pragma unroll
+          for (int s = 0; s < 2; s++) {
+            float g[32], w[32];
+            tmem_ld32x2(tbase + c0 + s * 32, tbase + OUT_N + c0 + s * 32, g, w);
+            if (bias) {
+              add_bias32<T>(g, bias, ocol + s * 32, args.n_out);
+              add_bias32<T>(w, bias + args.n_out, ocol + s * 32, args.n_out);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) v[s * 32 + i] = silu16(g[i]) * w[i];
+          }
+        } else {
+          tmem_ld32x2(tbase + c0, lo, hi);
+          if (bias) {
+            add_bias32<T>(lo, bias, ocol, args.n_out);
+            add_bias32<T>(hi, bias, ocol + 32, args.n_out);
+          }
+          if (args.act == FLETCHER_ACT_GELU) {
+#pragma unroll
+            for (int i = 0; i < 64; i++) v[i] = gelu_fast16(v[i]);
+          }
+        }
+        if (u == UNITS - 1) {  // every TMEM read of this tile is done: release the accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR)
+              mbar_arrive_cluster(tempty_lead + acc * 8);
+            else
+              mbar_arrive(&tempty[acc]);
+          }
+        }
+        if (ocol >= args.n_out || row0 >= t.end) continue;
+        if (row0 + 32 <= t.end) {
+          // 32 whole rows: staged in the swizzled box and stored by TMA, columns past the end clipped.
+          if (lane == 0) bulk_wait_read0();  // the box's last store has left it
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack8<T>(v + 8 * j);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC, box, (int)ocol, row0);
+            bulk_commit();
+          }
+        } else if (row0 + lane < t.end) {  // the group's last rows: the next rows are another group's
+          T* dst = out + (int64_t)(row0 + lane) * args.n_out + ocol;
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
+        }
+      }
+    }
+    if (lane == 0) bulk_wait0();
+  }
+
+  tc_fence_before();
+  if constexpr (PAIR)
+    cluster_sync();  // no cross-CTA signal or MMA is in flight past this point
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS)
+                   : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS)
+                   : "memory");
+  }
+}
+
+template <typename T, int BN, bool PAIR, bool GATED, bool GATHER>
+int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  using C = Cfg<BN, PAIR>;
+  constexpr int OUT_N = GATED ? BN / 2 : BN;
+  CUtensorMap ma, mb, mc;
+  int32_t rc;
+  if ((rc = make_tma_map_2d(c, &ma, dt, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.K, BK, GATHER ? 1 : BM)))
+    return rc;
+  if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
+  if ((rc = make_tma_map_2d(c, &mc, dt, g.out, (uint64_t)g.pairs, (uint64_t)g.n_out, (uint64_t)g.n_out, 64, 32)))
+    return rc;
+  Args a{};
+  a.offsets = g.offsets;
+  a.pair_of = g.pair_of;
+  a.bias = g.bias;
+  a.out = g.out;
+  a.err = c->d_err;
+  a.N = g.N;
+  a.n_out = g.n_out;
+  a.E = g.experts;
+  a.top_k = g.top_k;
+  a.num_kb = (int)((g.K + BK - 1) / BK);
+  a.n_tiles = (int)((g.n_out + OUT_N - 1) / OUT_N);
+  a.act = g.act;
+  auto kern = k_grouped_tc<T, BN, PAIR, GATED, GATHER>;
+  static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
+  if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
+    FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_set[c->device & 63].store(true, std::memory_order_release);
+  }
+  // At most this many row tiles, whatever the groups are.
+  const int64_t mt = g.pairs / C::TILE_M + std::min<int64_t>(g.experts, g.pairs);
+  const int64_t tiles = mt * a.n_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  const int units = PAIR ? c->num_sms / 2 : c->num_sms;
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, units) * (PAIR ? 2 : 1)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = c->stream;
+  cfg.attrs = at;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  FL_CUDA(c, cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, a));
+  FL_LAUNCH(c);
+  return FLETCHER_OK;
+}
+
+template <typename T, int BN, bool PAIR>
+int32_t pick(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  const bool gather = g.pair_of != nullptr;
+  if (g.act == FLETCHER_ACT_SWIGLU)
+    return gather ? run<T, BN, PAIR, true, true>(c, dt, g) : run<T, BN, PAIR, true, false>(c, dt, g);
+  return gather ? run<T, BN, PAIR, false, true>(c, dt, g) : run<T, BN, PAIR, false, false>(c, dt, g);
+}
+
+template <typename T>
+int32_t launch(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  // Pairs of SMs on 256 x 256 tiles where groups have rows for them on average; else 128-row tiles.
+  if (g.pairs >= 256 * (int64_t)g.experts) return pick<T, 256, true>(c, dt, g);
+  return pick<T, 256, false>(c, dt, g);
+}
+
+}  // namespace tcg
+
+bool grouped_tc_supported(int32_t dtype, const GroupedArgs& g) {
+  const uintptr_t ptrs = (uintptr_t)g.x | (uintptr_t)g.w | (uintptr_t)g.bias | (uintptr_t)g.out;
+  return dtype != FLETCHER_F32 && (ptrs & 15) == 0 && g.K % 8 == 0 && g.n_out % 8 == 0 && g.act != FLETCHER_ACT_TANH;
+}
+
+int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& g) {
+  if (dtype == FLETCHER_BF16) return tcg::launch<__nv_bfloat16>(c, dtype, g);
+  return tcg::launch<__half>(c, dtype, g);
+}
+
+}  // namespace fl

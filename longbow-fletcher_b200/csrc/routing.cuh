@@ -52,6 +52,8 @@ struct GroupedArgs {
   int64_t pairs;  // upper bound of the slots
   int32_t act;
 };
+bool grouped_tc_supported(int32_t dtype, const GroupedArgs& a);
+int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& a);
 int32_t launch_grouped_simt(Ctx* c, int32_t dtype, const GroupedArgs& a);
 
 }  // namespace fl
