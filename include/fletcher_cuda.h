@@ -252,8 +252,12 @@ int32_t Cuda_MeanPoolL2(CudaContextRef ctx, CudaBufferRef hidden, const int32_t*
  * chooses, products grouped by expert compute, a weighted sum joins, and the norms around the
  * block follow.  (The reference has the dense block only.)  Shared rules:
  *   - all calls enqueue on the context's stream, read sizes that depend on the routing on the
- *     device alone, allocate nothing and never wait for the GPU, so that a sequence of them can be
- *     captured into a CUDA graph (except Cuda_Routing_Assign, which reads host arrays);
+ *     device alone and never wait for the GPU, so that a sequence of them can be captured into a
+ *     CUDA graph (except Cuda_Routing_Assign, which reads host arrays);
+ *   - Cuda_Linear_Grouped of token rows keeps a workspace with its routing (up to rows * top_k *
+ *     inCols elements, at most doubled), which a call that needs more makes larger; earlier ones
+ *     stay valid until the routing is freed.  During a capture it cannot grow: the call fails, so
+ *     make it once before;
  *   - buffers are dense and row-major, and share one dtype except where noted;
  *   - an output may not overlap an input unless its entry below says so.
  *

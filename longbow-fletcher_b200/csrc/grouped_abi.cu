@@ -53,15 +53,23 @@ int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t
                   !overlap(y->ptr, ybytes, r->mem, r->bytes),
            "Linear_Grouped: the result overlaps an input");
   if (a.pairs == 0) return FLETCHER_OK;
-  touch(y);
   a.x = x->ptr;
   a.w = w->ptr;
   a.bias = b ? b->ptr : nullptr;
   a.out = y->ptr;
   a.offsets = r->offsets;
+  a.slots = inputOrder == FLETCHER_ROWS_TOKENS ? r->slots : nullptr;
   a.pair_of = inputOrder == FLETCHER_ROWS_TOKENS ? r->pair_of : nullptr;
   a.act = activation;
-  if (grouped_tc_supported(dt, a)) return launch_grouped_tc(c, dt, a);
+  if (grouped_tc_supported(dt, a)) {
+    void* ws = nullptr;
+    const int64_t need = grouped_tc_workspace(a);
+    const int32_t rc = need ? routing_workspace(r, need, &ws) : FLETCHER_OK;
+    if (rc) return rc;
+    touch(y);
+    return launch_grouped_tc(c, dt, a, ws);
+  }
+  touch(y);
   return launch_grouped_simt(c, dt, a);
 }
 

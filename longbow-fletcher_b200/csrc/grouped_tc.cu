@@ -2,8 +2,12 @@
 // out[s] = act(x[row(s)] . W[e] + b[e]), W [E][K, N] as the framework stores Linear weights,
 // (in, out).
 //
-// Layout: rows of x are K-major operands, fetched in 128-byte-swizzled 64-wide slabs: by TMA tiles
-// where a group's rows lie together, by TMA gathers of four rows where slots point at tokens.  W is
+// Layout: rows of x are K-major operands, TMA tiles in 128-byte-swizzled 64-wide slabs, in slot order:
+// rows of tokens are first copied there (k_place_rows), once, instead of being gathered again for
+// each column tile.  Gathering in the product itself was measured on 32768 tokens x 2 of 8 experts,
+// 768 -> 2 x 2048: 445 TFLOP/s with TMA gathers of four rows (80 cycles each), 760 with cp.async by
+// four warps (1450 cycles a 16 KB slab, whatever the rows' order), against 1250 from rows that lie
+// together.  W is
 // read as it is stored: its rows are K, its columns contiguous, so boxes of 64 K x 64 columns are
 // MN-major operands (64 columns = one 128-byte swizzle row, 8-row K groups 1024 bytes apart, column
 // blocks 8 KB apart).  No weight is packed or copied, and SwiGLU's gate and up columns are simply
@@ -64,30 +68,13 @@ struct Cfg {
 
 struct Args {
   const int32_t* offsets;
-  const int32_t* pair_of;
   const void* bias;
   void* out;
   int32_t* err;
   int64_t N, n_out;
-  int32_t E, top_k, num_kb, n_tiles, act;
+  int32_t E, num_kb, n_tiles, act;
 };
 
-// Four rows of a 2-D tensor by index (64 columns from x), one below the other.
-template <bool PAIR>
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint32_t bar, int x, const int (&r)[4]) {
-  if constexpr (PAIR)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(bar), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-        : "memory");
-}
 template <bool PAIR>
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
   if constexpr (PAIR)
@@ -179,10 +166,10 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 
-// Persistent: warp 0 loads (TMA tiles or gathers), warp 1 issues the MMAs and owns the TMEM, warps 2-9
-// drain one accumulator while the next tile fills the other.  As the dense GEMM: bounded waits, and
+// Persistent: warp 0 loads by TMA, warp 1 issues the MMAs and owns the TMEM, warps 2-9 drain one
+// accumulator while the next tile fills the other.  As the dense GEMM: bounded waits, and
 // on expiry every role leaves after what it issued has landed.
-template <typename T, int BN, bool PAIR, bool GATED, bool GATHER>
+template <typename T, int BN, bool PAIR, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
     k_grouped_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const Args args) {
@@ -250,71 +237,44 @@ __global__ void __launch_bounds__(kThreads, 1)
   Walk walk{args.offsets, prefix, args.n_tiles, C::TILE_M};
 
   if (warp == 0) {
-    // Producer: lane 0 loads tiles; in a gather every lane fetches its own four rows.
-    int stage = 0;
-    uint32_t phase = 0, issued = 0, issued_par = 0;
-    int rows[4] = {}, next[4] = {};
-    auto fetch = [&](const Tile& t, int (&r)[4]) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int s = t.first + (int)crank * BM + 4 * lane + i;
-        r[i] = args.pair_of[s < t.end ? s : t.first];  // rows past the group are computed, not stored
-      }
-    };
-    Tile cur{};
-    if (first_tile < num_tiles) {
-      cur = walk.at(first_tile);
-      if constexpr (GATHER) fetch(cur, next);
-    }
-    bool ok = true;
-    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
-      const Tile t = cur;
-      if constexpr (GATHER) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) rows[i] = next[i] / args.top_k;
-      }
-      if (tile + tile_stride < num_tiles) {  // the next tile's rows are on their way during this one
-        cur = walk.at(tile + tile_stride);
-        if constexpr (GATHER) fetch(cur, next);
-      }
-      const int a_row = t.first + (int)crank * BM;
-      for (int kb = 0; kb < args.num_kb; kb++) {
-        ok = GATHER || lane == 0 ? mbar_wait_spin(&empty[stage], phase ^ 1, abort, args.err) : true;
-        if constexpr (GATHER) ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        uint8_t* a = sA + stage * C::A_BYTES;
-        uint8_t* b = sB + stage * C::B_BYTES;
-        // In a pair both CTAs' loads complete on the even CTA's barrier, which expects both.
-        const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
-        if (lane == 0) {
-          if (crank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * C::STAGE_BYTES);
-          if constexpr (!GATHER) {
-            if constexpr (PAIR)
-              tma_load_2d_pair(a, &tmA, fb, kb * BK, a_row);
-            else
-              tma_load_2d(a, &tmA, &full[stage], kb * BK, a_row);
-          }
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, issued_par = 0;
+      // In a pair both CTAs' loads complete on the even CTA's barrier, which expects both.
+      constexpr uint32_t kBytes = (PAIR ? 2 : 1) * C::STAGE_BYTES;
+      bool ok = true;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
+        const Tile t = walk.at(tile);
+        for (int kb = 0; kb < args.num_kb; kb++) {
+          if (!(ok = mbar_wait_spin(&empty[stage], phase ^ 1, abort, args.err))) break;
+          uint8_t* a = sA + stage * C::A_BYTES;
+          uint8_t* b = sB + stage * C::B_BYTES;
+          const uint32_t fb = PAIR ? mapa_shared(smem_u32(&full[stage]), 0) : smem_u32(&full[stage]);
+          if (crank == 0) mbar_expect_tx(&full[stage], kBytes);
+          if constexpr (PAIR)
+            tma_load_2d_pair(a, &tmA, fb, kb * BK, t.first + (int)crank * BM);
+          else
+            tma_load_2d(a, &tmA, &full[stage], kb * BK, t.first);
 #pragma unroll
           for (int i = 0; i < C::B_COLS / 64; i++) {
             const int col = i * 64 + (int)crank * C::B_COLS;  // accumulator column
             const int x = GATED ? t.nb * OUT_N + col % OUT_N + (col >= OUT_N ? (int)args.n_out : 0) : t.nb * BN + col;
             tma_load_3d<PAIR>(b + i * kColBlock, &tmB, fb, x, kb * BK, t.e);
           }
-        }
-        if constexpr (GATHER) tma_gather4<PAIR>(a + lane * 512, &tmA, fb, kb * BK, rows);
-        issued |= 1u << stage;
-        issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
-        if (++stage == C::STAGES) {
-          stage = 0;
-          phase ^= 1;
+          issued |= 1u << stage;
+          issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
       }
+      // Leaving early: the loads in flight land before the CTA exits (in a pair they complete on the even
+      // CTA's barriers; the odd CTA cannot pass the last cluster barrier before that one has seen them).
+      if (*abort && crank == 0)
+        for (int s = 0; s < C::STAGES; s++)
+          if ((issued >> s) & 1) mbar_drain(&full[s], (issued_par >> s) & 1);
     }
-    // Leaving early: the loads in flight land before the CTA exits (in a pair they complete on the even
-    // CTA's barriers; the odd CTA cannot pass the last cluster barrier before that one has seen them).
-    if (lane == 0 && *abort && crank == 0)
-      for (int s = 0; s < C::STAGES; s++)
-        if ((issued >> s) & 1) mbar_drain(&full[s], (issued_par >> s) & 1);
   } else if (warp == 1) {
     if (lane == 0 && crank == 0) {
       const uint32_t id = idesc<T, C::TILE_M, BN, true>();
@@ -386,11 +346,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         float v[64];
         float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
         float (&hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
+        auto release = [&]() {  // every TMEM read of this tile is done
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (PAIR)
+              mbar_arrive_cluster(tempty_lead + acc * 8);
+            else
+              mbar_arrive(&tempty[acc]);
+          }
+        };
         if constexpr (GATED) {
 #pragma unroll
           for (int s = 0; s < 2; s++) {
             float g[32], w[32];
             tmem_ld32x2(tbase + c0 + s * 32, tbase + OUT_N + c0 + s * 32, g, w);
+            if (u == UNITS - 1 && s == 1) release();
             if (bias) {
               add_bias32<T>(g, bias, ocol + s * 32, args.n_out);
               add_bias32<T>(w, bias + args.n_out, ocol + s * 32, args.n_out);
@@ -400,6 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           tmem_ld32x2(tbase + c0, lo, hi);
+          if (u == UNITS - 1) release();
           if (bias) {
             add_bias32<T>(lo, bias, ocol, args.n_out);
             add_bias32<T>(hi, bias, ocol + 32, args.n_out);
@@ -407,16 +379,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (args.act == FLETCHER_ACT_GELU) {
 #pragma unroll
             for (int i = 0; i < 64; i++) v[i] = gelu_fast16(v[i]);
-          }
-        }
-        if (u == UNITS - 1) {  // every TMEM read of this tile is done: release the accumulator
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (PAIR)
-              mbar_arrive_cluster(tempty_lead + acc * 8);
-            else
-              mbar_arrive(&tempty[acc]);
           }
         }
         if (ocol >= args.n_out || row0 >= t.end) continue;
@@ -460,31 +422,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <typename T, int BN, bool PAIR, bool GATED, bool GATHER>
+template <typename T, int BN, bool PAIR, bool GATED>
 int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
   using C = Cfg<BN, PAIR>;
   constexpr int OUT_N = GATED ? BN / 2 : BN;
   CUtensorMap ma, mb, mc;
   int32_t rc;
-  if ((rc = make_tma_map_2d(c, &ma, dt, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.K, BK, GATHER ? 1 : BM)))
+  if ((rc = make_tma_map_2d(c, &ma, dt, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.K, BK, BM)))
     return rc;
   if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
   if ((rc = make_tma_map_2d(c, &mc, dt, g.out, (uint64_t)g.pairs, (uint64_t)g.n_out, (uint64_t)g.n_out, 64, 32)))
     return rc;
   Args a{};
   a.offsets = g.offsets;
-  a.pair_of = g.pair_of;
   a.bias = g.bias;
   a.out = g.out;
   a.err = c->d_err;
   a.N = g.N;
   a.n_out = g.n_out;
   a.E = g.experts;
-  a.top_k = g.top_k;
   a.num_kb = (int)((g.K + BK - 1) / BK);
   a.n_tiles = (int)((g.n_out + OUT_N - 1) / OUT_N);
   a.act = g.act;
-  auto kern = k_grouped_tc<T, BN, PAIR, GATED, GATHER>;
+  auto kern = k_grouped_tc<T, BN, PAIR, GATED>;
   static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
   if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
     FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
@@ -515,10 +475,34 @@ int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
 
 template <typename T, int BN, bool PAIR>
 int32_t pick(Ctx* c, int32_t dt, const GroupedArgs& g) {
-  const bool gather = g.pair_of != nullptr;
-  if (g.act == FLETCHER_ACT_SWIGLU)
-    return gather ? run<T, BN, PAIR, true, true>(c, dt, g) : run<T, BN, PAIR, true, false>(c, dt, g);
-  return gather ? run<T, BN, PAIR, false, true>(c, dt, g) : run<T, BN, PAIR, false, false>(c, dt, g);
+  return g.act == FLETCHER_ACT_SWIGLU ? run<T, BN, PAIR, true>(c, dt, g) : run<T, BN, PAIR, false>(c, dt, g);
+}
+
+// Token rows copied to their slots: a warp a token, whose row is read once and written for each of its
+// choices.  Bound by HBM at (1 + top_k) * rows * K * 2 bytes.
+__global__ void __launch_bounds__(256) k_place_rows(const uint4* __restrict__ x, const int32_t* __restrict__ slots,
+                                                    int64_t rows, int top_k, int vecs, uint4* __restrict__ out) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  for (int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < rows;
+       t += ((int64_t)gridDim.x * blockDim.x) >> 5) {
+    const uint4* src = x + t * vecs;
+    const int mine = lane < top_k ? slots[t * top_k + lane] : -1;
+    for (int v0 = 0; v0 < vecs; v0 += 128) {
+      uint4 q[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (v0 + i * 32 + lane < vecs) q[i] = __ldcs(src + v0 + i * 32 + lane);
+      for (int j = 0; j < top_k; j++) {
+        const int slot = __shfl_sync(0xffffffffu, mine, j);
+        if (slot < 0) continue;
+        uint4* dst = out + (int64_t)slot * vecs + v0 + lane;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (v0 + i * 32 + lane < vecs) dst[i * 32] = q[i];
+      }
+    }
+  }
 }
 
 template <typename T>
@@ -535,7 +519,18 @@ bool grouped_tc_supported(int32_t dtype, const GroupedArgs& g) {
   return dtype != FLETCHER_F32 && (ptrs & 15) == 0 && g.K % 8 == 0 && g.n_out % 8 == 0 && g.act != FLETCHER_ACT_TANH;
 }
 
-int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& g) {
+int64_t grouped_tc_workspace(const GroupedArgs& g) { return g.slots ? g.pairs * g.K * 2 : 0; }
+
+int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& args, void* workspace) {
+  GroupedArgs g = args;
+  if (g.slots) {
+    const int64_t blocks = std::min<int64_t>((g.x_rows + 7) / 8, (int64_t)c->num_sms * 8);
+    FL_CUDA(c, launch_pdl(tcg::k_place_rows, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const uint4*)g.x, g.slots,
+                          g.x_rows, g.top_k, (int)(g.K / 8), (uint4*)workspace));
+    FL_LAUNCH(c);
+    g.x = workspace;
+    g.x_rows = g.pairs;
+  }
   if (dtype == FLETCHER_BF16) return tcg::launch<__nv_bfloat16>(c, dtype, g);
   return tcg::launch<__half>(c, dtype, g);
 }

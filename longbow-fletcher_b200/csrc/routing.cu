@@ -312,6 +312,31 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
 }
 
 }  // namespace
+
+int32_t routing_workspace(Routing* r, int64_t bytes, void** out) {
+  Ctx* c = r->c;
+  const int n = r->num_work;
+  if (n == 0 || r->work_bytes[n - 1] < bytes) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    FL_CUDA(c, cudaStreamIsCapturing(c->stream, &st));
+    FL_CHECK(c, st == cudaStreamCaptureStatusNone,
+             "Linear_Grouped: the routing's workspace must grow; make the call once before capturing it");
+    FL_CHECK(c, n < Routing::kMaxBlocks, "Linear_Grouped: the routing's workspace cannot grow further");
+    // Twice the last block: what was outgrown adds up to less than the newest.
+    const int64_t want = std::max(bytes, n ? 2 * r->work_bytes[n - 1] : 0);
+    int32_t rc = dev_alloc(c, &r->work[n], want);
+    r->work_bytes[n] = want;
+    if (rc && want > bytes) {
+      rc = dev_alloc(c, &r->work[n], bytes);
+      r->work_bytes[n] = bytes;
+    }
+    if (rc) return rc;
+    r->num_work++;
+  }
+  *out = r->work[r->num_work - 1];
+  return FLETCHER_OK;
+}
+
 }  // namespace fl
 
 using namespace fl;
@@ -361,6 +386,7 @@ int32_t Cuda_Routing_Free(CudaRoutingRef routing) {
   if (!r) return FLETCHER_OK;
   DeviceGuard g(r->c);
   dev_free(r->c, r->mem, r->bytes);
+  for (int i = 0; i < r->num_work; i++) dev_free(r->c, r->work[i], r->work_bytes[i]);
   delete r;
   return FLETCHER_OK;
 }

@@ -22,8 +22,17 @@ struct Routing {
   int32_t* pair_of = nullptr;  // [pairs] pair of each slot; behind the last slot unspecified
   int32_t* offsets = nullptr;  // [num_experts + 1]
   int32_t* hist = nullptr;     // [blocks, num_experts] choices of each expert in a block's rows
+  // Cuda_Linear_Grouped's copy of token rows in slot order, grown on demand.  Blocks that were outgrown
+  // stay until the routing is freed: captured graphs may still use them.
+  static constexpr int kMaxBlocks = 48;
+  void* work[kMaxBlocks] = {};
+  int64_t work_bytes[kMaxBlocks] = {};
+  int num_work = 0;
   int64_t pairs() const { return rows * top_k; }
 };
+
+// At least `bytes` of the routing's workspace; may allocate, but not while the stream is captured.
+int32_t routing_workspace(Routing* r, int64_t bytes, void** out);
 
 inline Routing* as_routing(CudaRoutingRef r) { return reinterpret_cast<Routing*>(r); }
 
@@ -47,13 +56,15 @@ struct GroupedArgs {
   int64_t K, N, n_out;
   int64_t x_rows;          // rows of x
   const int32_t* offsets;  // [experts + 1]
-  const int32_t* pair_of;  // rows of x are tokens: slot s reads row pair_of[s] / top_k; null: row s
+  const int32_t* slots;    // rows of x are tokens: [tokens, top_k] slots of each; null: rows are slots
+  const int32_t* pair_of;  // with `slots`, the inverse: slot s reads row pair_of[s] / top_k
   int32_t top_k, experts;
   int64_t pairs;  // upper bound of the slots
   int32_t act;
 };
 bool grouped_tc_supported(int32_t dtype, const GroupedArgs& a);
-int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& a);
+int64_t grouped_tc_workspace(const GroupedArgs& a);  // bytes
+int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& a, void* workspace);
 int32_t launch_grouped_simt(Ctx* c, int32_t dtype, const GroupedArgs& a);
 
 }  // namespace fl
