@@ -104,61 +104,115 @@ __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const f
   }
 }
 
+// A row's inputs are asked for one row ahead: the next y (or the first kAhead choices' rows, whose slots
+// are asked for two rows ahead) while this row is normed, the next residual once this one is used.
+constexpr int kAhead = 2;
 template <typename T, int NV, int WPR, bool COMBINE>
-__global__ void __launch_bounds__(kThreads) k_block_norm(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, NV > 2 ? 2 : 3) k_block_norm(const NormArgs a) {
   constexpr int VEC = 16 / sizeof(T), TPR = 32 * WPR, TEAMS = kThreads / TPR;
+  constexpr int NY = COMBINE ? kAhead : 1;
   __shared__ float red[kTurns][8];
   int turn = 0;
-  const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+  const int lane = threadIdx.x & 31, t = threadIdx.x % TPR, team = threadIdx.x / TPR;
   const int nvec = a.cols / VEC;
-  pdl_wait();
-  for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < a.rows; row += (int64_t)gridDim.x * TEAMS) {
-    float v[NV * VEC];
-    auto add = [&](const T* src, float scale, bool first) {
-      Pack<T> p[NV];
+  const int64_t step = (int64_t)gridDim.x * TEAMS;
+  int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+  Pack<T> py[NY][NV], pr[NV];
+  auto load = [&](Pack<T> (&p)[NV], const void* base, int64_t r) {
+    const uint4* src = reinterpret_cast<const uint4*>(base) + r * nvec + t;
 #pragma unroll
-      for (int j = 0; j < NV; j++)
-        if (j * TPR + t < nvec) p[j].q = *reinterpret_cast<const uint4*>(src + (int64_t)(j * TPR + t) * VEC);
-#pragma unroll
-      for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          const float f = j * TPR + t < nvec ? to_f<T>(p[j].t[i]) : 0.f;
-          v[j * VEC + i] = first ? scale * f : fmaf(scale, f, v[j * VEC + i]);
-        }
-    };
+    for (int j = 0; j < NV; j++)
+      if (j * TPR + t < nvec) p[j].q = src[j * TPR];
+  };
+  // Combine: lane j < top_k holds choice j of the current and of the next row.
+  int32_t slot = -1, slot_next = -1;
+  float w = 0.f, w_next = 0.f;
+  auto load_slot = [&](int64_t r, int32_t& s, float& f) {
+    s = -1;
+    if (r < a.rows && lane < a.top_k) {
+      s = a.slots[r * a.top_k + lane];
+      f = a.weights[r * a.top_k + lane];
+    }
+  };
+  auto load_y = [&](int64_t r, int32_t s) {
     if constexpr (COMBINE) {
 #pragma unroll
-      for (int i = 0; i < NV * VEC; i++) v[i] = 0.f;
-      for (int j = 0; j < a.top_k; j++) {
-        const int32_t slot = a.slots[row * a.top_k + j];
-        if (slot >= 0) add(reinterpret_cast<const T*>(a.y) + (int64_t)slot * a.cols, a.weights[row * a.top_k + j], false);
+      for (int j = 0; j < NY; j++) {
+        const int32_t sj = __shfl_sync(0xffffffffu, s, j);  // -1 past the choices
+        if (sj >= 0) load(py[j], a.y, sj);
       }
-    } else {
-      add(reinterpret_cast<const T*>(a.y) + row * a.cols, 1.0f, true);
+    } else if (r < a.rows) {
+      load(py[0], a.y, r);
     }
+  };
+  pdl_wait();
+  if constexpr (COMBINE) {
+    load_slot(row, slot, w);
+    load_slot(row + step, slot_next, w_next);
+  }
+  load_y(row, slot);
+  if (a.residual && row < a.rows) load(pr, a.residual, row);
+  for (; row < a.rows; row += step) {
+    float v[NV * VEC];
+    auto add = [&](const Pack<T> (&p)[NV], float scale) {
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (j * TPR + t < nvec) {
+#pragma unroll
+          for (int i = 0; i < VEC; i++) v[j * VEC + i] = fmaf(scale, to_f<T>(p[j].t[i]), v[j * VEC + i]);
+        }
+    };
+    Pack<T> pg[NV];
+    if (a.gate) {
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_step) + t;
+#pragma unroll
+      for (int j = 0; j < NV; j++)
+        if (j * TPR + t < nvec) pg[j].q = src[j * TPR];
+    }
+#pragma unroll
+    for (int i = 0; i < NV * VEC; i++) v[i] = 0.f;
+    if constexpr (COMBINE) {
+#pragma unroll
+      for (int j = 0; j < NY; j++) {
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        if (__shfl_sync(0xffffffffu, slot, j) >= 0) add(py[j], wj);
+      }
+      for (int j = NY; j < a.top_k; j++) {
+        const int32_t sj = __shfl_sync(0xffffffffu, slot, j);
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        if (sj >= 0) {
+          load(py[0], a.y, sj);
+          add(py[0], wj);
+        }
+      }
+      slot = slot_next;
+      w = w_next;
+      load_slot(row + 2 * step, slot_next, w_next);
+    } else {
+      add(py[0], 1.0f);
+    }
+    load_y(row + step, slot);
     norm_row<VEC, NV, WPR>(v, a.post, a.post_gamma, a.post_beta, a.eps, t, nvec, a.cols, red, turn);
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-      if (a.gate && j * TPR + t < nvec) {
-        Pack<T> g;
-        g.q = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_step +
-                                              (int64_t)(j * TPR + t) * VEC);
+    for (int j = 0; j < NV; j++)
 #pragma unroll
-        for (int i = 0; i < VEC; i++) v[j * VEC + i] *= to_f<T>(g.t[i]);
+      for (int i = 0; i < VEC; i++) {
+        if (a.gate && j * TPR + t < nvec) v[j * VEC + i] *= to_f<T>(pg[j].t[i]);
+        v[j * VEC + i] *= a.branch_scale;
       }
-#pragma unroll
-      for (int i = 0; i < VEC; i++) v[j * VEC + i] *= a.branch_scale;
+    if (a.residual) {
+      add(pr, a.residual_scale);
+      if (row + step < a.rows) load(pr, a.residual, row + step);
     }
-    if (a.residual) add(reinterpret_cast<const T*>(a.residual) + row * a.cols, a.residual_scale, false);
     auto store = [&](void* to) {
+      uint4* dst = reinterpret_cast<uint4*>(to) + row * nvec + t;
 #pragma unroll
       for (int j = 0; j < NV; j++) {
         if (j * TPR + t < nvec) {
           Pack<T> o;
 #pragma unroll
           for (int i = 0; i < VEC; i++) o.t[i] = from_f<T>(v[j * VEC + i]);
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(to) + row * a.cols + (int64_t)(j * TPR + t) * VEC) = o.q;
+          dst[j * TPR] = o.q;
         }
       }
     };
@@ -241,7 +295,7 @@ __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs 
 template <typename T, int NV, int WPR, bool COMBINE>
 int32_t launch_vec(Ctx* c, const NormArgs& a) {
   constexpr int TEAMS = kThreads / (32 * WPR);
-  const int64_t blocks = std::min<int64_t>((a.rows + TEAMS - 1) / TEAMS, (int64_t)c->num_sms * 8);
+  const int64_t blocks = std::min<int64_t>((a.rows + TEAMS - 1) / TEAMS, (int64_t)c->num_sms * (NV > 2 ? 2 : 3));
   FL_CUDA(c, launch_pdl(k_block_norm<T, NV, WPR, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
