@@ -68,37 +68,43 @@ __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const f
                                          float (*red)[8], int& turn) {
   constexpr int TPR = 32 * WPR;
   if (kind == FLETCHER_NORM_NONE) return;
-  float s = 0.f, mean = 0.f;
+  // In packed pairs of fp32: half the instructions, which at 16-bit widths weigh as much as the bytes.
+  float s0 = 0.f, s1 = 0.f, mean = 0.f;
   if (kind == FLETCHER_NORM_LAYER) {
 #pragma unroll
-    for (int i = 0; i < NV * VEC; i++) s += v[i];
-    mean = team_sum<WPR>(s, red, turn) / (float)cols;
-    s = 0.f;
+    for (int i = 0; i < NV * VEC; i += 2) add2(s0, s1, v[i], v[i + 1]);
+    mean = team_sum<WPR>(s0 + s1, red, turn) / (float)cols;
+    s0 = s1 = 0.f;
   }
 #pragma unroll
   for (int j = 0; j < NV; j++) {
     if (j * TPR + t < nvec) {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        v[j * VEC + i] -= mean;
-        s = fmaf(v[j * VEC + i], v[j * VEC + i], s);
+      for (int i = j * VEC; i < (j + 1) * VEC; i += 2) {
+        if (kind == FLETCHER_NORM_LAYER) add2(v[i], v[i + 1], -mean, -mean);
+        fma2(s0, s1, v[i], v[i + 1], v[i], v[i + 1], s0, s1);
       }
     }
   }
-  const float inv = 1.0f / sqrtf(team_sum<WPR>(s, red, turn) / (float)cols + eps);
+  const float inv = 1.0f / sqrtf(team_sum<WPR>(s0 + s1, red, turn) / (float)cols + eps);
 #pragma unroll
   for (int j = 0; j < NV; j++) {
     const int at = j * TPR + t;
     if (at < nvec) {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
-        float4 g = gamma ? __ldg(reinterpret_cast<const float4*>(gamma + at * VEC + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
-        float4 b = beta ? __ldg(reinterpret_cast<const float4*>(beta + at * VEC + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
         float* p = &v[j * VEC + i];
-        p[0] = fmaf(p[0] * inv, g.x, b.x);
-        p[1] = fmaf(p[1] * inv, g.y, b.y);
-        p[2] = fmaf(p[2] * inv, g.z, b.z);
-        p[3] = fmaf(p[3] * inv, g.w, b.w);
+        mul2(p[0], p[1], p[0], p[1], inv, inv);
+        mul2(p[2], p[3], p[2], p[3], inv, inv);
+        const float4 g = gamma ? __ldg(reinterpret_cast<const float4*>(gamma + at * VEC + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
+        if (beta) {
+          const float4 b = __ldg(reinterpret_cast<const float4*>(beta + at * VEC + i));
+          fma2(p[0], p[1], p[0], p[1], g.x, g.y, b.x, b.y);
+          fma2(p[2], p[3], p[2], p[3], g.z, g.w, b.z, b.w);
+        } else {
+          mul2(p[0], p[1], p[0], p[1], g.x, g.y);
+          mul2(p[2], p[3], p[2], p[3], g.z, g.w);
+        }
       }
     }
   }
@@ -107,8 +113,12 @@ __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const f
 // A row's inputs are asked for one row ahead: the next y (or the first kAhead choices' rows, whose slots
 // are asked for two rows ahead) while this row is normed, the next residual once this one is used.
 constexpr int kAhead = 2;
+// Blocks an SM, by the registers that a row's vectors need (two choices' rows and a residual in flight).
+// 16384 x 8 x 768 combine: 55 us with 2, 50 with 3; 65536 x 768 norms: 78 with 2, 90 with 3, which spills.
+template <int NV, bool COMBINE>
+constexpr int kMinBlocks = NV == 1 ? 4 : NV == 2 || (COMBINE && NV == 3) ? 3 : 2;
 template <typename T, int NV, int WPR, bool COMBINE>
-__global__ void __launch_bounds__(kThreads, NV > 2 ? 2 : 3) k_block_norm(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, kMinBlocks<NV, COMBINE>) k_block_norm(const NormArgs a) {
   constexpr int VEC = 16 / sizeof(T), TPR = 32 * WPR, TEAMS = kThreads / TPR;
   constexpr int NY = COMBINE ? kAhead : 1;
   __shared__ float red[kTurns][8];
@@ -159,7 +169,10 @@ __global__ void __launch_bounds__(kThreads, NV > 2 ? 2 : 3) k_block_norm(const N
       for (int j = 0; j < NV; j++)
         if (j * TPR + t < nvec) {
 #pragma unroll
-          for (int i = 0; i < VEC; i++) v[j * VEC + i] = fmaf(scale, to_f<T>(p[j].t[i]), v[j * VEC + i]);
+          for (int i = 0; i < VEC; i += 2) {
+            float* o = &v[j * VEC + i];
+            fma2(o[0], o[1], to_f<T>(p[j].t[i]), to_f<T>(p[j].t[i + 1]), scale, scale, o[0], o[1]);
+          }
         }
     };
     Pack<T> pg[NV];
@@ -193,13 +206,21 @@ __global__ void __launch_bounds__(kThreads, NV > 2 ? 2 : 3) k_block_norm(const N
     }
     load_y(row + step, slot);
     norm_row<VEC, NV, WPR>(v, a.post, a.post_gamma, a.post_beta, a.eps, t, nvec, a.cols, red, turn);
+    if (a.gate) {
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+      for (int j = 0; j < NV; j++)
+        if (j * TPR + t < nvec) {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        if (a.gate && j * TPR + t < nvec) v[j * VEC + i] *= to_f<T>(pg[j].t[i]);
-        v[j * VEC + i] *= a.branch_scale;
-      }
+          for (int i = 0; i < VEC; i += 2) {
+            float* o = &v[j * VEC + i];
+            mul2(o[0], o[1], o[0], o[1], to_f<T>(pg[j].t[i]), to_f<T>(pg[j].t[i + 1]));
+          }
+        }
+    }
+    if (a.branch_scale != 1.0f) {
+#pragma unroll
+      for (int i = 0; i < NV * VEC; i += 2) mul2(v[i], v[i + 1], v[i], v[i + 1], a.branch_scale, a.branch_scale);
+    }
     if (a.residual) {
       add(pr, a.residual_scale);
       if (row + step < a.rows) load(pr, a.residual, row + step);
@@ -295,7 +316,10 @@ __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs 
 template <typename T, int NV, int WPR, bool COMBINE>
 int32_t launch_vec(Ctx* c, const NormArgs& a) {
   constexpr int TEAMS = kThreads / (32 * WPR);
-  const int64_t blocks = std::min<int64_t>((a.rows + TEAMS - 1) / TEAMS, (int64_t)c->num_sms * (NV > 2 ? 2 : 3));
+  // As few teams as walk the rows in the same number of turns.
+  const int64_t most = (int64_t)c->num_sms * kMinBlocks<NV, COMBINE> * TEAMS;
+  const int64_t turns = (a.rows + most - 1) / most;
+  const int64_t blocks = (a.rows + turns * TEAMS - 1) / (turns * TEAMS);
   FL_CUDA(c, launch_pdl(k_block_norm<T, NV, WPR, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;

@@ -68,11 +68,12 @@ struct Cfg {
 
 struct Args {
   const int32_t* offsets;
+  const int32_t* pair_of;  // k_grouped_small: slot s reads row pair_of[s] / top_k
   const void* bias;
   void* out;
   int32_t* err;
   int64_t N, n_out;
-  int32_t E, num_kb, n_tiles, act;
+  int32_t E, top_k, num_kb, n_tiles, act;
 };
 
 template <bool PAIR>
@@ -422,6 +423,265 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- few rows a group
+// Few rows a group: the weights' bytes are the work, so a tile takes at most 32 rows of x (4 KB a slab next
+// to 16 KB of W; the MMA's other 96 rows read whatever lies behind and are never looked at), rows of
+// tokens are gathered by TMA in quads, only as many as there are, and the rest of shared memory is a
+// deep ring of W.  Warps 0 and 4 drain lanes 0-31 of the accumulator, half the columns each.
+struct SmallCfg {
+  static constexpr int TILE_M = 32, BN = 128;
+  static constexpr int kThreads = 160;
+  static constexpr int A_BYTES = TILE_M * BK * 2;
+  static constexpr int B_BYTES = BN * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = 11;
+  static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
+  static constexpr int TABLE_OFF = BAR_OFF + 384;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int SMEM = TABLE_OFF + (kMaxExperts + 1 + 32) * 4 + 1024;
+  static_assert((2 * STAGES + 8) * 8 <= 384, "barrier area");
+  static_assert(SMEM <= 232448, "shared memory budget");
+  static_assert(STAGES * B_BYTES >= BM * BK * 2, "the MMA reads 128 rows from the last slab of x on");
+};
+
+// Four rows of a 2-D tensor by index, 64 columns from x, one below the other.
+__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint64_t* bar, int x, const int (&r)[4]) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+      : "memory");
+}
+
+template <typename T, bool GATED, bool GATHER>
+__global__ void __launch_bounds__(SmallCfg::kThreads, 1)
+    k_grouped_small(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
+  using C = SmallCfg;
+  constexpr int BN = C::BN, OUT_N = GATED ? BN / 2 : BN;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + C::STAGES * C::A_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint64_t* drain = tempty + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem + C::TABLE_OFF);
+  int32_t* tmp = prefix + kMaxExperts + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 32) {
+    for (int i = 0; i < C::STAGES; i++) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 2);
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmA) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmB) : "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_holder)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();  // the routing and x are the previous kernels' work
+  fill_table(args.offsets, args.E, C::TILE_M, prefix, tmp);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const int num_tiles = prefix[args.E] * args.n_tiles;
+  Walk walk{args.offsets, prefix, args.n_tiles, C::TILE_M};
+
+  if (warp == 1) {
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, issued_par = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const Tile t = walk.at(tile);
+      const int quads = GATHER ? (min(t.end - t.first, C::TILE_M) + 3) / 4 : 0;
+      int rows[4] = {};
+      if (GATHER && lane < quads) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int s = t.first + 4 * lane + i;
+          rows[i] = args.pair_of[s < t.end ? s : t.first] / args.top_k;  // past the group: computed, not stored
+        }
+      }
+      for (int kb = 0; kb < args.num_kb; kb++) {
+        ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[stage], phase ^ 1, abort, args.err));
+        if (!ok) break;
+        uint8_t* a = sA + stage * C::A_BYTES;
+        uint8_t* b = sB + stage * C::B_BYTES;
+        if (lane == 0) {
+          mbar_expect_tx(&full[stage], C::B_BYTES + (GATHER ? quads * 512 : C::A_BYTES));
+#pragma unroll
+          for (int i = 0; i < BN / 64; i++) {
+            const int x = GATED ? t.nb * OUT_N + i * (int)args.n_out : t.nb * BN + i * 64;
+            tma_load_3d<false>(b + i * kColBlock, &tmB, smem_u32(&full[stage]), x, kb * BK, t.e);
+          }
+          if constexpr (!GATHER) tma_load_2d(a, &tmA, &full[stage], kb * BK, t.first);
+        }
+        if (GATHER && lane < quads) tma_gather4(a + lane * 512, &tmA, &full[stage], kb * BK, rows);
+        issued |= 1u << stage;
+        issued_par = (issued_par & ~(1u << stage)) | (phase << stage);
+        if (++stage == C::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (lane == 0 && *abort)  // leaving early: the loads in flight land before the CTA exits
+      for (int s = 0; s < C::STAGES; s++)
+        if ((issued >> s) & 1) mbar_drain(&full[s], (issued_par >> s) & 1);
+  } else if (warp == 2) {
+    if (lane == 0) {
+      const uint32_t id = idesc<T, BM, BN, true>();
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+        const int acc = it & 1;
+        if (!mbar_wait_spin(&tempty[acc], ((it >> 1) & 1) ^ 1, abort, args.err)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * BN;
+        for (int kb = 0; kb < args.num_kb; kb++) {
+          if (!(ok = mbar_wait_spin(&full[stage], phase, abort, args.err))) break;
+          tc_fence_after();
+          const uint64_t da = sw128_desc(smem_u32(sA + stage * C::A_BYTES));
+          const uint64_t db = desc_mn(smem_u32(sB + stage * C::B_BYTES));
+#pragma unroll
+          for (int k = 0; k < BK / 16; k++)
+            mma_f16(d, da + 2 * k, db + (uint64_t)k * (2048 >> 4), id, (kb | k) != 0);
+          mma_commit(&empty[stage]);
+          if (++stage == C::STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        mma_commit(&tfull[acc]);
+      }
+      if (*abort) {
+        mma_commit(drain);
+        mbar_drain(drain, 0);
+      }
+    }
+  } else if (warp == 0 || warp == 4) {
+    const int half = warp >> 2;
+    constexpr int COLS = OUT_N / 2;  // this warp's output columns: 32 (gated) or 64
+    T* out = reinterpret_cast<T*>(args.out);
+    int it = 0;
+    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
+      const Tile t = walk.at(tile);
+      const int acc = it & 1;
+      const uint32_t tbase = tmem_base + acc * BN;
+      const T* bias = args.bias ? reinterpret_cast<const T*>(args.bias) + (int64_t)t.e * args.N : nullptr;
+      if (!mbar_wait_spin(&tfull[acc], (it >> 1) & 1, abort, args.err)) break;
+      tc_fence_after();
+      const int c0 = half * COLS;
+      const int64_t ocol = (int64_t)t.nb * OUT_N + c0;
+      float v[64];
+      float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
+      float (&hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
+      tmem_ld32x2(tbase + c0, tbase + c0 + (GATED ? OUT_N : 32), lo, hi);  // gated: gate and up
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[acc]);
+      if (bias) {
+        add_bias32<T>(lo, bias, ocol, args.n_out);
+        if constexpr (GATED)
+          add_bias32<T>(hi, bias + args.n_out, ocol, args.n_out);
+        else
+          add_bias32<T>(hi, bias, ocol + 32, args.n_out);
+      }
+      if constexpr (GATED) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) v[i] = silu16(v[i]) * v[32 + i];
+      } else if (args.act == FLETCHER_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 64; i++) v[i] = gelu_fast16(v[i]);
+      }
+      if (t.first + lane < t.end) {
+        T* dst = out + (int64_t)(t.first + lane) * args.n_out + ocol;
+#pragma unroll
+        for (int j = 0; j < COLS / 8; j++)
+          if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS) : "memory");
+  }
+}
+
+Args args_of(const Ctx* c, const GroupedArgs& g, int out_n) {
+  Args a{};
+  a.offsets = g.offsets;
+  a.pair_of = g.pair_of;
+  a.top_k = g.top_k;
+  a.bias = g.bias;
+  a.out = g.out;
+  a.err = c->d_err;
+  a.N = g.N;
+  a.n_out = g.n_out;
+  a.E = g.experts;
+  a.num_kb = (int)((g.K + BK - 1) / BK);
+  a.n_tiles = (int)((g.n_out + out_n - 1) / out_n);
+  a.act = g.act;
+  return a;
+}
+
+// At most this many tiles, whatever the groups are.
+int64_t most_tiles(const GroupedArgs& g, int tile_m, int n_tiles) {
+  return (g.pairs / tile_m + std::min<int64_t>(g.experts, g.pairs)) * n_tiles;
+}
+
+template <typename T, bool GATED, bool GATHER>
+int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  using C = SmallCfg;
+  CUtensorMap ma, mb;
+  int32_t rc;
+  if ((rc = make_tma_map_2d(c, &ma, dt, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.K, BK,
+                            GATHER ? 1 : C::TILE_M)))
+    return rc;
+  if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
+  const Args a = args_of(c, g, GATED ? C::BN / 2 : C::BN);
+  auto kern = k_grouped_small<T, GATED, GATHER>;
+  static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
+  if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
+    FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_set[c->device & 63].store(true, std::memory_order_release);
+  }
+  const int64_t grid = std::min<int64_t>(most_tiles(g, C::TILE_M, a.n_tiles), c->num_sms);
+  FL_CUDA(c, launch_pdl(kern, dim3((unsigned)grid), dim3(C::kThreads), C::SMEM, c->stream, ma, mb, a));
+  FL_LAUNCH(c);
+  return FLETCHER_OK;
+}
+
+template <typename T>
+int32_t launch_small(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  const bool gather = g.pair_of != nullptr;
+  if (g.act == FLETCHER_ACT_SWIGLU)
+    return gather ? run_small<T, true, true>(c, dt, g) : run_small<T, true, false>(c, dt, g);
+  return gather ? run_small<T, false, true>(c, dt, g) : run_small<T, false, false>(c, dt, g);
+}
+
 template <typename T, int BN, bool PAIR, bool GATED>
 int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
   using C = Cfg<BN, PAIR>;
@@ -433,26 +693,14 @@ int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
   if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
   if ((rc = make_tma_map_2d(c, &mc, dt, g.out, (uint64_t)g.pairs, (uint64_t)g.n_out, (uint64_t)g.n_out, 64, 32)))
     return rc;
-  Args a{};
-  a.offsets = g.offsets;
-  a.bias = g.bias;
-  a.out = g.out;
-  a.err = c->d_err;
-  a.N = g.N;
-  a.n_out = g.n_out;
-  a.E = g.experts;
-  a.num_kb = (int)((g.K + BK - 1) / BK);
-  a.n_tiles = (int)((g.n_out + OUT_N - 1) / OUT_N);
-  a.act = g.act;
+  const Args a = args_of(c, g, OUT_N);
   auto kern = k_grouped_tc<T, BN, PAIR, GATED>;
   static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
   if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
     FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_set[c->device & 63].store(true, std::memory_order_release);
   }
-  // At most this many row tiles, whatever the groups are.
-  const int64_t mt = g.pairs / C::TILE_M + std::min<int64_t>(g.experts, g.pairs);
-  const int64_t tiles = mt * a.n_tiles;
+  const int64_t tiles = most_tiles(g, C::TILE_M, a.n_tiles);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -519,10 +767,15 @@ bool grouped_tc_supported(int32_t dtype, const GroupedArgs& g) {
   return dtype != FLETCHER_F32 && (ptrs & 15) == 0 && g.K % 8 == 0 && g.n_out % 8 == 0 && g.act != FLETCHER_ACT_TANH;
 }
 
-int64_t grouped_tc_workspace(const GroupedArgs& g) { return g.slots ? g.pairs * g.K * 2 : 0; }
+// At most 32 rows an expert on average, counting no more experts than there are rows.
+static bool few_rows(const GroupedArgs& g) { return g.pairs <= 32 * std::min<int64_t>(g.experts, g.pairs); }
+
+int64_t grouped_tc_workspace(const GroupedArgs& g) { return g.slots && !few_rows(g) ? g.pairs * g.K * 2 : 0; }
 
 int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& args, void* workspace) {
   GroupedArgs g = args;
+  if (few_rows(g))
+    return dtype == FLETCHER_BF16 ? tcg::launch_small<__nv_bfloat16>(c, dtype, g) : tcg::launch_small<__half>(c, dtype, g);
   if (g.slots) {
     const int64_t blocks = std::min<int64_t>((g.x_rows + 7) / 8, (int64_t)c->num_sms * 8);
     FL_CUDA(c, launch_pdl(tcg::k_place_rows, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const uint4*)g.x, g.slots,
