@@ -159,6 +159,21 @@ __device__ __forceinline__ void add_bias32(float (&v)[32], const T* b, int64_t c
   }
 }
 
+// gelu_fast16 on two values in packed fp32.
+__device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
+  float a0, a1, u0, u1, q0, q1, n0, n1, d0, d1;
+  mul2(q0, q1, x0, x1, x0, x1);
+  mul2(a0, a1, x0, x1, 0.044715f, 0.044715f);
+  fma2(u0, u1, a0, a1, q0, q1, x0, x1);
+  mul2(u0, u1, u0, u1, 0.7978846f, 0.7978846f);
+  mul2(q0, q1, u0, u1, u0, u1);
+  fma2(n0, n1, q0, q1, u0, u1, 27.0f * u0, 27.0f * u1);
+  fma2(d0, d1, q0, q1, 9.0f, 9.0f, 27.0f, 27.0f);
+  const float p0 = __fdividef(n0, d0), p1 = __fdividef(n1, d1);
+  const float t0 = fabsf(u0) > 4.0f ? copysignf(1.0f, u0) : p0, t1 = fabsf(u1) > 4.0f ? copysignf(1.0f, u1) : p1;
+  mul2(x0, x1, x0, x1, 0.5f, 0.5f);
+  fma2(x0, x1, x0, x1, t0, t1, x0, x1);
+}
 __device__ __forceinline__ float silu16(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
 
 // Row-per-lane 64 values -> 16-byte chunks of T.
@@ -326,8 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Epilogue: warps 2-5 take the first half of a tile's output columns, warps 6-9 the second; warp w
     // reads TMEM lanes 32 * (w % 4) .., its lanes' rows.
     const int q = warp & 3, half = (warp - 2) >> 2;
-    constexpr int UNITS = OUT_N / 128;  // 64-column units of a warp
-    static_assert(UNITS >= 1, "tile width");
+    constexpr int UW = OUT_N >= 128 ? 64 : 32, UNITS = OUT_N / 2 / UW;  // a warp's units of UW columns
     uint8_t* box = smem + C::OUT_OFF + (warp - 2) * kBox;
     const uint32_t tempty_lead = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0;
     T* out = reinterpret_cast<T*>(args.out);
@@ -342,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
 #pragma unroll 1
       for (int u = 0; u < UNITS; u++) {
-        const int c0 = half * (OUT_N / 2) + u * 64;  // first output column of the unit within the tile
+        const int c0 = half * (OUT_N / 2) + u * UW;  // first output column of the unit within the tile
         const int64_t ocol = (int64_t)t.nb * OUT_N + c0;
         float v[64];
         float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
@@ -359,10 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if constexpr (GATED) {
 #pragma unroll
-          for (int s = 0; s < 2; s++) {
+          for (int s = 0; s < UW / 32; s++) {
             float g[32], w[32];
             tmem_ld32x2(tbase + c0 + s * 32, tbase + OUT_N + c0 + s * 32, g, w);
-            if (u == UNITS - 1 && s == 1) release();
+            if (u == UNITS - 1 && s == UW / 32 - 1) release();
             if (bias) {
               add_bias32<T>(g, bias, ocol + s * 32, args.n_out);
               add_bias32<T>(w, bias + args.n_out, ocol + s * 32, args.n_out);
@@ -379,11 +393,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (args.act == FLETCHER_ACT_GELU) {
 #pragma unroll
-            for (int i = 0; i < 64; i++) v[i] = gelu_fast16(v[i]);
+            for (int i = 0; i < 64; i += 2) gelu_pair(v[i], v[i + 1]);
           }
         }
         if (ocol >= args.n_out || row0 >= t.end) continue;
-        if (row0 + 32 <= t.end) {
+        if (UW == 64 && row0 + 32 <= t.end) {
           // 32 whole rows: staged in the swizzled box and stored by TMA, columns past the end clipped.
           if (lane == 0) bulk_wait_read0();  // the box's last store has left it
           __syncwarp();
@@ -399,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (row0 + lane < t.end) {  // the group's last rows: the next rows are another group's
           T* dst = out + (int64_t)(row0 + lane) * args.n_out + ocol;
 #pragma unroll
-          for (int j = 0; j < 8; j++)
+          for (int j = 0; j < UW / 8; j++)
             if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
         }
       }
@@ -611,7 +625,7 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
         for (int i = 0; i < 32; i++) v[i] = silu16(v[i]) * v[32 + i];
       } else if (args.act == FLETCHER_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < 64; i++) v[i] = gelu_fast16(v[i]);
+        for (int i = 0; i < 64; i += 2) gelu_pair(v[i], v[i + 1]);
       }
       if (t.first + lane < t.end) {
         T* dst = out + (int64_t)(t.first + lane) * args.n_out + ocol;
@@ -755,8 +769,17 @@ __global__ void __launch_bounds__(256) k_place_rows(const uint4* __restrict__ x,
 
 template <typename T>
 int32_t launch(Ctx* c, int32_t dt, const GroupedArgs& g) {
-  // Pairs of SMs on 256 x 256 tiles where groups have rows for them on average; else 128-row tiles.
-  if (g.pairs >= 256 * (int64_t)g.experts) return pick<T, 256, true>(c, dt, g);
+  const bool gated = g.act == FLETCHER_ACT_SWIGLU;
+  // 256 accumulator columns keep the tensor core fed (with 128 it reads x's rows from shared memory
+  // for half the work: 32000 x 6 of 64 experts, 1024 -> 2 x 704, 678 against 552 us); 128 where all
+  // tiles run at once either way, so that twice the SMs work (1536 of 12 experts, 776 -> 1000: 11.6
+  // against 15.5 us).
+  const int64_t groups = std::min<int64_t>(g.experts, g.pairs);
+  const int64_t tiles = (2 * g.pairs / BM + groups) * ((g.n_out + (gated ? 63 : 127)) / (gated ? 64 : 128)) / 2;
+  if (tiles <= c->num_sms) return pick<T, 128, false>(c, dt, g);
+  // Pairs of SMs on 256 x 256 tiles where groups have rows for them on average (12000 x 2 of 8 experts,
+  // 768 -> 2 x 2048: 134 against 147 us with 128 x 256; 128 rows an expert, 64 experts: 58 against 49).
+  if (g.pairs >= 256 * groups) return pick<T, 256, true>(c, dt, g);
   return pick<T, 256, false>(c, dt, g);
 }
 
@@ -767,23 +790,33 @@ bool grouped_tc_supported(int32_t dtype, const GroupedArgs& g) {
   return dtype != FLETCHER_F32 && (ptrs & 15) == 0 && g.K % 8 == 0 && g.n_out % 8 == 0 && g.act != FLETCHER_ACT_TANH;
 }
 
-// At most 32 rows an expert on average, counting no more experts than there are rows.
-static bool few_rows(const GroupedArgs& g) { return g.pairs <= 32 * std::min<int64_t>(g.experts, g.pairs); }
+// Rows an expert on average, counting no more experts than there are rows, decide between the kernels.
+// Measured with weights from HBM, 768 -> 2 x 2048 of 8 and 1024 -> 2 x 704 of 64 experts, us:
+//   rows an expert                         4            8            16           32
+//   32-row tiles, rows gathered in them    12.8  37.8   13.6  41.6   15.1  45.7   23.9  67.4
+//   32-row tiles, rows placed before       14.2  37.2   14.0  37.9   14.0  38.1   17.2  48.1
+//   128-row tiles, rows placed before      15.3  39.5   15.2  41.1   14.3  41.6   14.3  42.4
+static bool rows_per_expert_at_most(const GroupedArgs& g, int n) {
+  return g.pairs <= n * std::min<int64_t>(g.experts, g.pairs);
+}
+static bool gathers(const GroupedArgs& g) { return g.slots && rows_per_expert_at_most(g, 4); }
 
-int64_t grouped_tc_workspace(const GroupedArgs& g) { return g.slots && !few_rows(g) ? g.pairs * g.K * 2 : 0; }
+int64_t grouped_tc_workspace(const GroupedArgs& g) { return g.slots && !gathers(g) ? g.pairs * g.K * 2 : 0; }
 
 int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& args, void* workspace) {
   GroupedArgs g = args;
-  if (few_rows(g))
-    return dtype == FLETCHER_BF16 ? tcg::launch_small<__nv_bfloat16>(c, dtype, g) : tcg::launch_small<__half>(c, dtype, g);
-  if (g.slots) {
+  const bool small = rows_per_expert_at_most(g, 16);
+  if (g.slots && !gathers(g)) {
     const int64_t blocks = std::min<int64_t>((g.x_rows + 7) / 8, (int64_t)c->num_sms * 8);
     FL_CUDA(c, launch_pdl(tcg::k_place_rows, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const uint4*)g.x, g.slots,
                           g.x_rows, g.top_k, (int)(g.K / 8), (uint4*)workspace));
     FL_LAUNCH(c);
     g.x = workspace;
     g.x_rows = g.pairs;
+    g.slots = g.pair_of = nullptr;
   }
+  if (small)
+    return dtype == FLETCHER_BF16 ? tcg::launch_small<__nv_bfloat16>(c, dtype, g) : tcg::launch_small<__half>(c, dtype, g);
   if (dtype == FLETCHER_BF16) return tcg::launch<__nv_bfloat16>(c, dtype, g);
   return tcg::launch<__half>(c, dtype, g);
 }
