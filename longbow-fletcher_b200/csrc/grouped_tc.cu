@@ -104,24 +104,21 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
   return d;
 }
 
-// The groups' row tiles: prefix[e] tiles come before group e's.  Filled by the whole block.
-__device__ __forceinline__ void fill_table(const int32_t* offsets, int E, int tile_m, int32_t* prefix, int32_t* tmp) {
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+// Copies the offsets to shared memory and counts the groups' row tiles; by the whole block.
+__device__ __forceinline__ int fill_table(const int32_t* offsets, int E, int tile_m, int32_t* offs, int32_t* tmp) {
+  const int t = threadIdx.x, warp = t >> 5, warps = blockDim.x >> 5;
   int n = 0;
-  if (t < E) n = (offsets[t + 1] - offsets[t] + tile_m - 1) / tile_m;
-  int s = n;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
+  for (int e = t; e <= E; e += blockDim.x) {
+    const int o = offsets[e];
+    offs[e] = o;
+    if (e < E) n += (offsets[e + 1] - o + tile_m - 1) / tile_m;
   }
-  if (lane == 31) tmp[warp] = s;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((t & 31) == 0) tmp[warp] = n;
   __syncthreads();
-  int before = 0;
-  for (int w = 0; w < warp; w++) before += tmp[w];
-  if (t < E) prefix[t + 1] = before + s;
-  if (t == 0) prefix[0] = 0;
-  __syncthreads();
+  n = 0;
+  for (int w = 0; w < warps; w++) n += tmp[w];
+  return n;
 }
 
 struct Tile {
@@ -129,17 +126,15 @@ struct Tile {
 };
 // Tiles are asked for in ascending order.
 struct Walk {
-  const int32_t *offsets, *prefix;
-  int n_tiles, tile_m, e = -1, first = 0, end = 0;
+  const int32_t* offs;
+  int n_tiles, tile_m, e = 0, before = 0;  // row tiles of the experts before e
   __device__ __forceinline__ Tile at(int tile) {
     const int mt = tile / n_tiles;
-    if (e < 0 || prefix[e + 1] <= mt) {
-      do e++;
-      while (prefix[e + 1] <= mt);
-      first = offsets[e];
-      end = offsets[e + 1];
+    for (;; e++) {
+      const int first = offs[e], end = offs[e + 1], n = (end - first + tile_m - 1) / tile_m;
+      if (mt < before + n) return {e, first + (mt - before) * tile_m, end, tile - mt * n_tiles};
+      before += n;
     }
-    return {e, first + (mt - prefix[e]) * tile_m, end, tile - mt * n_tiles};
   }
 };
 
@@ -176,6 +171,8 @@ __device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
 }
 __device__ __forceinline__ float silu16(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
 
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // Row-per-lane 64 values -> 16-byte chunks of T.
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float* v) {
@@ -203,8 +200,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  int32_t* prefix = reinterpret_cast<int32_t*>(smem + C::TABLE_OFF);
-  int32_t* tmp = prefix + kMaxExperts + 1;
+  int32_t* offs = reinterpret_cast<int32_t*>(smem + C::TABLE_OFF);
+  int32_t* tmp = offs + kMaxExperts + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = PAIR ? cluster_ctarank() : 0;
@@ -241,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   pdl_wait();  // the routing and x are the previous kernels' work
-  fill_table(args.offsets, args.E, C::TILE_M, prefix, tmp);
+  const int num_tiles = fill_table(args.offsets, args.E, C::TILE_M, offs, tmp) * args.n_tiles;
   tc_fence_before();
   if constexpr (PAIR)
     cluster_sync();  // both CTAs' barriers are initialised before any cross-CTA signal
@@ -249,8 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  const int num_tiles = prefix[args.E] * args.n_tiles;
-  Walk walk{args.offsets, prefix, args.n_tiles, C::TILE_M};
+  Walk walk{offs, args.n_tiles, C::TILE_M};
 
   if (warp == 0) {
     if (lane == 0) {
@@ -352,6 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row0 = t.first + (int)crank * BM + q * 32;
       const uint32_t tbase = tmem_base + ((uint32_t)(q * 32) << 16) + acc * BN;
       const T* bias = args.bias ? reinterpret_cast<const T*>(args.bias) + (int64_t)t.e * args.N : nullptr;
+      if (bias && lane < 2 * UNITS) {  // a 128-byte line a unit, and one of the up columns
+        const int64_t col = (int64_t)t.nb * OUT_N + half * (OUT_N / 2) + (lane >> 1) * UW;
+        if (col < args.n_out && (GATED || (lane & 1) == 0)) prefetch_l1(bias + col + (lane & 1) * args.n_out);
+      }
       if (!mbar_wait_spin(&tfull[acc], (it >> 1) & 1, abort, args.err)) break;
       tc_fence_after();
 #pragma unroll 1
@@ -484,8 +484,8 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  int32_t* prefix = reinterpret_cast<int32_t*>(smem + C::TABLE_OFF);
-  int32_t* tmp = prefix + kMaxExperts + 1;
+  int32_t* offs = reinterpret_cast<int32_t*>(smem + C::TABLE_OFF);
+  int32_t* tmp = offs + kMaxExperts + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 32) {
@@ -510,13 +510,12 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();  // the routing and x are the previous kernels' work
-  fill_table(args.offsets, args.E, C::TILE_M, prefix, tmp);
+  const int num_tiles = fill_table(args.offsets, args.E, C::TILE_M, offs, tmp) * args.n_tiles;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  const int num_tiles = prefix[args.E] * args.n_tiles;
-  Walk walk{args.offsets, prefix, args.n_tiles, C::TILE_M};
+  Walk walk{offs, args.n_tiles, C::TILE_M};
 
   if (warp == 1) {
     int stage = 0;

@@ -1,11 +1,13 @@
 // Routing of rows to experts: top-k choice, weights, and the order of the choices by expert.
 //
 // A row's E logits lie in V = 8 consecutive values per lane of a group of G lanes (G the power of
-// two >= E / 8, at most a warp), so one or two vector loads a lane read the row and k rounds of
-// (8 compares + log2 G shuffles) find its choices.  A candidate is one 64-bit key: the logit's bits
-// in an order that compares like the value, above the complement of the expert's index, so the
-// largest key is the largest logit and, among equals, the lowest expert; round j takes the largest
-// key below round j-1's.  Exponentials use the first winner as the maximum.
+// two >= E / 8, at most a warp), so one or two vector loads a lane read the row.  A candidate is one
+// integer key: the logit's bits in an order that compares like the value, above the complement of the
+// expert's index, so the largest key is the largest logit and, among equals, the lowest expert (32
+// bits for 16-bit logits, else 64).  Each lane sorts its eight keys once (19 exchanges); a round
+// then takes the largest of the lanes' first keys (log2 G shuffles) and its owner moves on, where
+// comparing all eight again would cost 24 operations a round.  Lane j mod G keeps choice j and
+// computes its exponential, with the first winner as the maximum.
 //
 // Grouping is a stable counting sort in two launches without atomics on memory: k_route leaves, per
 // block of rows, how many choices each expert got; k_group sums the blocks before its own (and all
@@ -24,19 +26,57 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBlocksPerSM = 2;
 constexpr int V = 8;  // logits per lane
-typedef unsigned long long u64;
+// Keys.  0 for what is never chosen: -inf and NaN; +0 and -0 are equal.
+template <typename T>
+struct KeyOf {  // f32
+  typedef unsigned long long K;
+  static __device__ __forceinline__ K make(float x, int e) {
+    if (!(x > -INFINITY)) return 0;
+    if (x == 0.0f) x = 0.0f;
+    const uint32_t b = __float_as_uint(x);
+    return ((K)((b & 0x80000000u) ? ~b : b | 0x80000000u) << 32) | (uint32_t)~e;
+  }
+  static __device__ __forceinline__ int expert(K k) { return (int)~(uint32_t)k; }
+  static __device__ __forceinline__ float value(K k) {
+    const uint32_t o = (uint32_t)(k >> 32);
+    return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
+  }
+};
+template <typename T>
+struct KeyOf16 {
+  typedef uint32_t K;
+  static __device__ __forceinline__ K make(T x, int e) {
+    const float f = to_f<T>(x);
+    if (!(f > -INFINITY)) return 0;
+    const uint32_t b = f == 0.0f ? 0 : *reinterpret_cast<const uint16_t*>(&x);
+    return (((b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u) << 16) | (uint32_t)(0xffff - e);
+  }
+  static __device__ __forceinline__ int expert(K k) { return 0xffff - (int)(k & 0xffffu); }
+  static __device__ __forceinline__ float value(K k) {
+    const uint32_t o = k >> 16;
+    const uint16_t b = (uint16_t)((o & 0x8000u) ? o & 0x7fffu : ~o);
+    return to_f<T>(*reinterpret_cast<const T*>(&b));
+  }
+};
+template <>
+struct KeyOf<__half> : KeyOf16<__half> {};
+template <>
+struct KeyOf<__nv_bfloat16> : KeyOf16<__nv_bfloat16> {};
 
-// The value's bits as an unsigned integer that orders like the value; +0 and -0 are equal.
-// 0 for what is never chosen: -inf and NaN.
-__device__ __forceinline__ uint32_t ordered(float x) {
-  if (!(x > -INFINITY)) return 0;
-  if (x == 0.0f) x = 0.0f;
-  const uint32_t b = __float_as_uint(x);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(u64 key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
+// Eight keys in descending order.
+template <typename K>
+__device__ __forceinline__ void sort8(K (&k)[8]) {
+  auto ex = [&](int i, int j) {
+    const K hi = k[i] > k[j] ? k[i] : k[j], lo = k[i] > k[j] ? k[j] : k[i];
+    k[i] = hi;
+    k[j] = lo;
+  };
+  ex(0, 1), ex(2, 3), ex(4, 5), ex(6, 7);
+  ex(0, 2), ex(1, 3), ex(4, 6), ex(5, 7);
+  ex(1, 2), ex(5, 6);
+  ex(0, 4), ex(1, 5), ex(2, 6), ex(3, 7);
+  ex(2, 4), ex(3, 5);
+  ex(1, 2), ex(3, 4), ex(5, 6);
 }
 
 struct RouteArgs {
@@ -60,77 +100,92 @@ __device__ __forceinline__ float exp_below(float x, float m) { return x == m ? 1
 // The choices and weights of rows [r0, r1), and into `hist` (shared) each expert's count.
 template <typename T, int G>
 __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r1, int32_t* hist) {
-  const int lane = threadIdx.x & 31, gl = lane & (G - 1);
+  typedef KeyOf<T> Key;
+  typedef typename Key::K K;
+  constexpr int KEEP = (kMaxTopK + G - 1) / G;  // choices a lane keeps
+  constexpr int kPass = kThreads / G;
+  const int lane = threadIdx.x & 31, gl = lane & (G - 1), e0 = gl * V;
   const T* z = reinterpret_cast<const T*>(a.logits);
   const bool vec = a.E % V == 0 && ((uintptr_t)z & 15) == 0;
-  constexpr int kPass = kThreads / G;
+  union Row {
+    uint4 q[sizeof(T) * V / 16];
+    T t[V];
+  };
   // Whole groups step together; a group past the end works on the last row and writes nothing.
-  for (int64_t base = r0; base < r1; base += kPass) {
-    const int64_t mine = base + threadIdx.x / G;
-    const bool live = mine < r1;
-    const T* row = z + (live ? mine : r1 - 1) * a.E;
-    float x[V];
-    const int e0 = gl * V;
-    if (vec && e0 < a.E) {
-      union {
-        uint4 q[sizeof(T) * V / 16];
-        T t[V];
-      } u;
+  auto load = [&](int64_t r, Row& u) {
+    const T* row = z + (r < r1 ? r : r1 - 1) * a.E + e0;
+    if (vec) {
+      if (e0 < a.E) {
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(T) * V / 16); i++) u.q[i] = reinterpret_cast<const uint4*>(row + e0)[i];
-#pragma unroll
-      for (int i = 0; i < V; i++) x[i] = to_f<T>(u.t[i]);
+        for (int i = 0; i < (int)(sizeof(T) * V / 16); i++) u.q[i] = __ldg(reinterpret_cast<const uint4*>(row) + i);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < V; i++) x[i] = e0 + i < a.E ? to_f<T>(row[e0 + i]) : -INFINITY;
+      for (int i = 0; i < V; i++)
+        if (e0 + i < a.E) u.t[i] = row[i];
     }
-    u64 key[V];
+  };
+  Row next;
+  load(r0 + threadIdx.x / G, next);
+  for (int64_t base = r0; base < r1; base += kPass) {
+    const int64_t mine = base + threadIdx.x / G;
+    const Row cur = next;
+    if (base + kPass < r1) load(mine + kPass, next);  // on its way while this row is sorted
+    K key[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-      const uint32_t o = ordered(x[i]);
-      key[i] = o ? ((u64)o << 32) | (uint32_t)~(e0 + i) : 0;
+    for (int i = 0; i < V; i++) key[i] = e0 + i < a.E ? Key::make(cur.t[i], e0 + i) : 0;
+    const bool all = !a.sigmoid && !a.normalise;  // the weights' sum is over the whole row
+    float x[V];
+    if (all) {
+#pragma unroll
+      for (int i = 0; i < V; i++) x[i] = key[i] ? to_f<T>(cur.t[i]) : -INFINITY;
     }
-    u64 prev = ~0ull;
-    float m = 0.f, total = 0.f, w[kMaxTopK];
-    int id[kMaxTopK];
+    sort8(key);
+    float m = 0.f;
+    K kept[KEEP] = {};
 #pragma unroll
     for (int j = 0; j < kMaxTopK; j++) {
       if (j < a.k) {
-        u64 best = 0;
-#pragma unroll
-        for (int i = 0; i < V; i++)
-          if (key[i] < prev && key[i] > best) best = key[i];
+        K best = key[0];
 #pragma unroll
         for (int o = 1; o < G; o <<= 1) {
-          const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
-          if (other > best) best = other;
+          const K other = __shfl_xor_sync(0xffffffffu, best, o);
+          best = other > best ? other : best;
         }
-        prev = best;
-        const float v = value_of(best);
-        if (j == 0) m = v;
-        id[j] = best ? (int)~(uint32_t)best : -1;
-        w[j] = !best ? 0.f : a.sigmoid ? 1.0f / (1.0f + expf(-v)) : exp_below(v, m);
-        total += w[j];
+        if (key[0] == best) {  // keys are unique: one lane (or, at 0, lanes with nothing left)
+#pragma unroll
+          for (int i = 0; i + 1 < V; i++) key[i] = key[i + 1];
+          key[V - 1] = 0;
+        }
+        if (j == 0) m = Key::value(best);
+        if ((j & (G - 1)) == gl) kept[j / G] = best;
       }
     }
-    if (!a.sigmoid && !a.normalise) {
+    float w[KEEP], total = 0.f;
+#pragma unroll
+    for (int j = 0; j < KEEP; j++) {
+      const float v = Key::value(kept[j]);
+      w[j] = !kept[j] ? 0.f : a.sigmoid ? 1.0f / (1.0f + expf(-v)) : exp_below(v, m);
+      total += w[j];
+    }
+    if (all) {
       total = 0.f;
 #pragma unroll
       for (int i = 0; i < V; i++)
-        if (key[i]) total += exp_below(x[i], m);
-#pragma unroll
-      for (int o = 1; o < G; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (x[i] > -INFINITY) total += exp_below(x[i], m);
     }
-    const bool divide = !a.sigmoid || a.normalise;
-    if (live) {
 #pragma unroll
-      for (int j = 0; j < kMaxTopK; j++) {
-        if (j < a.k && (j & (G - 1)) == gl) {
-          float v = w[j];
-          if (divide) v = total > 0.f ? v / total : 0.f;
-          a.experts[mine * a.k + j] = id[j];
-          a.weights[mine * a.k + j] = v * a.scale;
-          if (id[j] >= 0) atomicAdd(&hist[id[j]], 1);
+    for (int o = 1; o < G; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const bool divide = !a.sigmoid || a.normalise;
+    if (mine < r1) {
+#pragma unroll
+      for (int i = 0; i < KEEP; i++) {
+        const int j = i * G + gl;
+        if (j < a.k) {
+          const int id = kept[i] ? Key::expert(kept[i]) : -1;
+          a.experts[mine * a.k + j] = id;
+          a.weights[mine * a.k + j] = (divide ? (total > 0.f ? w[i] / total : 0.f) : w[i]) * a.scale;
+          if (id >= 0) atomicAdd(&hist[id], 1);
         }
       }
     }
@@ -240,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArg
   const int share = kThreads / a.E, e = threadIdx.x % a.E, part = threadIdx.x / a.E;
   if (part < share) {
     int32_t b = 0, n = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int i = part; i < (int)gridDim.x; i += share) {
       const int32_t v = a.hist[(int64_t)i * a.E + e];
       n += v;
