@@ -1,13 +1,14 @@
 // Routing of rows to experts: top-k choice, weights, and the order of the choices by expert.
 //
-// A row's E logits lie in V = 8 consecutive values per lane of a group of G lanes (G the power of
-// two >= E / 8, at most a warp), so one or two vector loads a lane read the row.  A candidate is one
-// integer key: the logit's bits in an order that compares like the value, above the complement of the
-// expert's index, so the largest key is the largest logit and, among equals, the lowest expert (32
-// bits for 16-bit logits, else 64).  Each lane sorts its eight keys once (19 exchanges); a round
-// then takes the largest of the lanes' first keys (log2 G shuffles) and its owner moves on, where
-// comparing all eight again would cost 24 operations a round.  Lane j mod G keeps choice j and
-// computes its exponential, with the first winner as the maximum.
+// A row belongs to L lanes, which read its logits in chunks of eight.  A candidate is one integer key:
+// the logit's bits in an order that compares like the value, above the complement of the expert's
+// index, so the largest key is the largest logit and, among equals, the lowest expert (32 bits for
+// 16-bit logits, else 64).  Each lane keeps its KM >= top_k largest keys in order (a sorting network
+// for the first chunk, an insertion for each later key above the smallest); then a round takes the
+// largest of the lanes' first keys (log2 L shuffles) and its owner moves on.  Lane j mod L keeps
+// choice j and computes its exponential, with the first winner as the maximum.  Bound by instruction
+// issue: L = 4 lanes a row for many rows (65536 x 64 -> 6: 82 instructions a row, against 164 with 8
+// lanes that hold eight keys each), a whole warp a row where rows are few and latency counts.
 //
 // Grouping is a stable counting sort in two launches without atomics on memory: k_route leaves, per
 // block of rows, how many choices each expert got; k_group sums the blocks before its own (and all
@@ -65,12 +66,14 @@ struct KeyOf<__nv_bfloat16> : KeyOf16<__nv_bfloat16> {};
 
 // Eight keys in descending order.
 template <typename K>
+__device__ __forceinline__ void exchange(K& a, K& b) {
+  const K hi = a > b ? a : b, lo = a > b ? b : a;
+  a = hi;
+  b = lo;
+}
+template <typename K>
 __device__ __forceinline__ void sort8(K (&k)[8]) {
-  auto ex = [&](int i, int j) {
-    const K hi = k[i] > k[j] ? k[i] : k[j], lo = k[i] > k[j] ? k[j] : k[i];
-    k[i] = hi;
-    k[j] = lo;
-  };
+  auto ex = [&](int i, int j) { exchange(k[i], k[j]); };
   ex(0, 1), ex(2, 3), ex(4, 5), ex(6, 7);
   ex(0, 2), ex(1, 3), ex(4, 6), ex(5, 7);
   ex(1, 2), ex(5, 6);
@@ -94,25 +97,34 @@ struct RouteArgs {
   int32_t* hist;
 };
 
-// exp(x - m) where x may equal an infinite m.
-__device__ __forceinline__ float exp_below(float x, float m) { return x == m ? 1.0f : expf(x - m); }
+// exp(x - m) on the special-function unit, where x may equal an infinite m: the difference is rounded
+// once, its product with log2 e once more, so the relative error is about (|x - m| + 3) * 2^-24, and terms
+// far below the maximum, where that grows, are small.
+__device__ __forceinline__ float exp_below(float x, float m) {
+  const float t = x == m ? 0.0f : x - m;
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t * 1.44269504f));
+  return y;
+}
 
-// The choices and weights of rows [r0, r1), and into `hist` (shared) each expert's count.
-template <typename T, int G>
-__device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r1, int32_t* hist) {
+// The choices and weights of rows [r0, r1), into `hist` (shared) each expert's count, and, unless null,
+// the choices into `ids` (shared).
+template <typename T, int L, int KM>
+__device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r1, int32_t* hist, int16_t* ids) {
   typedef KeyOf<T> Key;
   typedef typename Key::K K;
-  constexpr int KEEP = (kMaxTopK + G - 1) / G;  // choices a lane keeps
-  constexpr int kPass = kThreads / G;
-  const int lane = threadIdx.x & 31, gl = lane & (G - 1), e0 = gl * V;
+  constexpr int KEEP = (KM + L - 1) / L;  // choices a lane keeps
+  constexpr int kPass = kThreads / L;
+  const int lane = threadIdx.x & 31, gl = lane & (L - 1);
+  const int chunks = (a.E + V * L - 1) / (V * L);
   const T* z = reinterpret_cast<const T*>(a.logits);
   const bool vec = a.E % V == 0 && ((uintptr_t)z & 15) == 0;
-  union Row {
+  union Chunk {
     uint4 q[sizeof(T) * V / 16];
     T t[V];
   };
-  // Whole groups step together; a group past the end works on the last row and writes nothing.
-  auto load = [&](int64_t r, Row& u) {
+  // Whole teams step together; a team past the end works on the last row and writes nothing.
+  auto load = [&](int64_t r, int e0, Chunk& u) {
     const T* row = z + (r < r1 ? r : r1 - 1) * a.E + e0;
     if (vec) {
       if (e0 < a.E) {
@@ -125,66 +137,102 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
         if (e0 + i < a.E) u.t[i] = row[i];
     }
   };
-  Row next;
-  load(r0 + threadIdx.x / G, next);
+  const bool all = !a.sigmoid && !a.normalise;  // the weights' sum is over the whole row
+  Chunk next;
+  load(r0 + threadIdx.x / L, gl * V, next);
   for (int64_t base = r0; base < r1; base += kPass) {
-    const int64_t mine = base + threadIdx.x / G;
-    const Row cur = next;
-    if (base + kPass < r1) load(mine + kPass, next);  // on its way while this row is sorted
-    K key[V];
+    const int64_t mine = base + threadIdx.x / L;
+    K list[KM] = {};
+    float lane_max = -INFINITY, lane_sum = 0.f;
+    for (int c = 0; c < chunks; c++) {
+      const int e0 = (c * L + gl) * V;
+      const Chunk cur = next;
+      if (c + 1 < chunks)  // on its way while this chunk is sorted
+        load(mine, e0 + L * V, next);
+      else if (base + kPass < r1)
+        load(mine + kPass, gl * V, next);
+      K key[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) key[i] = e0 + i < a.E ? Key::make(cur.t[i], e0 + i) : 0;
-    const bool all = !a.sigmoid && !a.normalise;  // the weights' sum is over the whole row
-    float x[V];
-    if (all) {
+      for (int i = 0; i < V; i++) key[i] = e0 + i < a.E ? Key::make(cur.t[i], e0 + i) : 0;
+      if (all) {  // running maximum and sum
+        float x[V], mx = lane_max;
 #pragma unroll
-      for (int i = 0; i < V; i++) x[i] = key[i] ? to_f<T>(cur.t[i]) : -INFINITY;
+        for (int i = 0; i < V; i++) {
+          x[i] = key[i] ? to_f<T>(cur.t[i]) : -INFINITY;
+          mx = fmaxf(mx, x[i]);
+        }
+        lane_sum *= exp_below(lane_max, mx);
+        lane_max = mx;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (key[i]) lane_sum += exp_below(x[i], mx);
+      }
+      if (KM >= V && c == 0) {
+        sort8(key);
+#pragma unroll
+        for (int i = 0; i < V; i++)
+          if (i < KM) list[i] = key[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          K k = key[i];
+          if (k > list[KM - 1]) {
+#pragma unroll
+            for (int j = 0; j < KM; j++) exchange(list[j], k);
+          }
+        }
+      }
     }
-    sort8(key);
     float m = 0.f;
     K kept[KEEP] = {};
+    if constexpr (L == 1) {
+      m = Key::value(list[0]);
 #pragma unroll
-    for (int j = 0; j < kMaxTopK; j++) {
-      if (j < a.k) {
-        K best = key[0];
+      for (int j = 0; j < KM; j++)
+        if (j < a.k) kept[j] = list[j];
+    } else {
 #pragma unroll
-        for (int o = 1; o < G; o <<= 1) {
-          const K other = __shfl_xor_sync(0xffffffffu, best, o);
-          best = other > best ? other : best;
+      for (int j = 0; j < KM; j++) {
+        if (j < a.k) {
+          K best = list[0];
+#pragma unroll
+          for (int o = 1; o < L; o <<= 1) {
+            const K other = __shfl_xor_sync(0xffffffffu, best, o);
+            best = other > best ? other : best;
+          }
+          const bool own = list[0] == best;  // keys are unique: one lane (or, at 0, lanes with nothing left)
+#pragma unroll
+          for (int i = 0; i < KM; i++) list[i] = own ? (i + 1 < KM ? list[i + 1] : 0) : list[i];
+          if (j == 0) m = Key::value(best);
+          if ((j & (L - 1)) == gl) kept[j / L] = best;
         }
-        if (key[0] == best) {  // keys are unique: one lane (or, at 0, lanes with nothing left)
-#pragma unroll
-          for (int i = 0; i + 1 < V; i++) key[i] = key[i + 1];
-          key[V - 1] = 0;
-        }
-        if (j == 0) m = Key::value(best);
-        if ((j & (G - 1)) == gl) kept[j / G] = best;
       }
     }
     float w[KEEP], total = 0.f;
 #pragma unroll
     for (int j = 0; j < KEEP; j++) {
-      const float v = Key::value(kept[j]);
-      w[j] = !kept[j] ? 0.f : a.sigmoid ? 1.0f / (1.0f + expf(-v)) : exp_below(v, m);
+      w[j] = 0.f;
+      if (kept[j]) {
+        const float v = Key::value(kept[j]);
+        w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-v)) : exp_below(v, m);
+      }
       total += w[j];
     }
-    if (all) {
-      total = 0.f;
+    if (all) total = lane_sum * exp_below(lane_max, m);
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (x[i] > -INFINITY) total += exp_below(x[i], m);
-    }
-#pragma unroll
-    for (int o = 1; o < G; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const bool divide = !a.sigmoid || a.normalise;
+    for (int o = 1; o < L; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    // Divided by the sum first, so that no product overflows before it; 0 where the sum is 0.
+    const float inv = a.sigmoid && !a.normalise ? 1.0f : total > 0.f ? __frcp_rn(total) : 0.f;
     if (mine < r1) {
+      const int64_t out = mine * a.k;
 #pragma unroll
       for (int i = 0; i < KEEP; i++) {
-        const int j = i * G + gl;
+        const int j = i * L + gl;
         if (j < a.k) {
           const int id = kept[i] ? Key::expert(kept[i]) : -1;
-          a.experts[mine * a.k + j] = id;
-          a.weights[mine * a.k + j] = (divide ? (total > 0.f ? w[i] / total : 0.f) : w[i]) * a.scale;
+          a.experts[out + j] = id;
+          a.weights[out + j] = w[i] * inv * a.scale;
+          if (ids) ids[(int)(out - r0 * a.k) + j] = (int16_t)id;
           if (id >= 0) atomicAdd(&hist[id], 1);
         }
       }
@@ -192,42 +240,61 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
   }
 }
 
-// Slots of the pairs [p0, p1).  start[e] (shared): the first slot of expert e in this block.
-// count (shared): [kWarps][E].
-__device__ __forceinline__ void assign_slots(const RouteArgs& a, int64_t p0, int64_t p1, const int32_t* start,
+// Slots of n <= kSub pairs from p0, whose experts are in ids (shared).  start[e] (shared): the first slot
+// of expert e, moved on by what is assigned.  count (shared): [kWarps][E].  Each warp ranks a run of pairs
+// against its own counters, the counters become the warps' first slots, and the ranks are added.
+constexpr int kSub = 4096, kRun = kSub / kWarps / 32;
+__device__ __forceinline__ void assign_slots(const RouteArgs& a, int64_t p0, int n, const int16_t* ids, int32_t* start,
                                              int32_t* count) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kWarps * a.E; i += kThreads) count[i] = 0;
-  __syncthreads();
-  const int64_t per = ((p1 - p0 + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int64_t w0 = p0 + warp * per, w1 = w0 + per < p1 ? w0 + per : p1;
+  const int per = ((n + kWarps - 1) / kWarps + 31) / 32 * 32, warps = (n + per - 1) / per;
+  const int w0 = warp * per;
   int32_t* mine = count + warp * a.E;
-  for (int64_t p = w0 + lane; p < w1; p += 32) {
-    const int e = a.experts[p];
-    if (e >= 0) atomicAdd(&mine[e], 1);
+  int rank[kRun];
+  if (warp < warps) {
+    for (int e = lane; e < a.E; e += 32) mine[e] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kRun; i++) {
+      if (i * 32 < per) {
+        const int p = w0 + i * 32 + lane;
+        const int e = p < n ? ids[p] : -1;
+        // The lanes with the same expert, bit by bit (__match_any_sync: three times the instructions).
+        uint32_t same = __ballot_sync(0xffffffffu, e >= 0);
+        for (int b = 0; (a.E - 1) >> b; b++) {
+          const uint32_t ones = __ballot_sync(0xffffffffu, (e >> b) & 1);
+          same &= (e >> b) & 1 ? ones : ~ones;
+        }
+        rank[i] = -1;
+        if (e >= 0) rank[i] = mine[e] + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (e >= 0 && lane == 31 - __clz(same)) mine[e] = rank[i] + 1;
+        __syncwarp();
+      }
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += kThreads) {
     int32_t at = start[e];
-    for (int w = 0; w < kWarps; w++) {
-      const int32_t n = count[w * a.E + e];
+    for (int w = 0; w < warps; w++) {
+      const int32_t c = count[w * a.E + e];
       count[w * a.E + e] = at;
-      at += n;
+      at += c;
     }
+    start[e] = at;
   }
   __syncthreads();
-  for (int64_t b = w0; b < w1; b += 32) {
-    const int64_t p = b + lane;
-    const int e = p < w1 ? a.experts[p] : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    int32_t slot = -1;
-    if (e >= 0) slot = mine[e] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (e >= 0 && lane == 31 - __clz(same)) mine[e] = slot + 1;
-    __syncwarp();
-    if (p < w1) {
-      a.slots[p] = slot;
-      if (slot >= 0) a.pair_of[slot] = (int32_t)p;
+  if (warp < warps) {
+#pragma unroll
+    for (int i = 0; i < kRun; i++) {
+      if (i * 32 < per) {
+        const int p = w0 + i * 32 + lane;
+        if (p < n) {
+          const int slot = rank[i] < 0 ? -1 : mine[ids[p]] + rank[i];
+          a.slots[p0 + p] = slot;
+          if (slot >= 0) a.pair_of[slot] = (int32_t)(p0 + p);
+        }
+      }
     }
   }
 }
@@ -253,20 +320,23 @@ __device__ __forceinline__ int32_t scan_experts(const int32_t* n, int32_t* at, i
   return total;
 }
 
-// ONE: a single block, which groups its pairs too.
-template <typename T, int G, bool ONE>
+// ONE: a single block, which groups its (at most kSub) pairs too.
+template <typename T, int L, int KM, bool ONE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArgs a) {
   __shared__ int32_t hist[kMaxExperts];
+  extern __shared__ int32_t dyn[];  // ONE: count [kWarps][E], ids [kSub]
+  int16_t* ids = ONE ? reinterpret_cast<int16_t*>(dyn + kWarps * a.E) : nullptr;
   for (int e = threadIdx.x; e < a.E; e += kThreads) hist[e] = 0;
   __syncthreads();
   pdl_wait();
   const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
   if (r0 < r1) {
     if (a.logits) {
-      choose<T, G>(a, r0, r1, hist);
+      choose<T, L, KM>(a, r0, r1, hist, ids);
     } else {
       for (int64_t p = r0 * a.k + threadIdx.x; p < r1 * a.k; p += kThreads) {
         const int e = a.experts[p];
+        if (ONE) ids[p] = (int16_t)e;
         if (e >= 0) atomicAdd(&hist[e], 1);
       }
     }
@@ -274,74 +344,102 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
   __syncthreads();
   if constexpr (ONE) {
     __shared__ int32_t at[kMaxExperts], tmp[kWarps + 1];
-    extern __shared__ int32_t count[];
     const int32_t total = scan_experts(hist, at, a.E, tmp);
     for (int e = threadIdx.x; e < a.E; e += kThreads) a.offsets[e] = at[e];
     if (threadIdx.x == 0) a.offsets[a.E] = total;
-    assign_slots(a, r0 * a.k, r1 * a.k, at, count);
+    assign_slots(a, 0, (int)(r1 * a.k), ids, at, dyn);
   } else {
-    for (int e = threadIdx.x; e < a.E; e += kThreads) a.hist[(int64_t)blockIdx.x * a.E + e] = hist[e];
+    for (int e = threadIdx.x; e < a.E; e += kThreads) a.hist[(int64_t)e * gridDim.x + blockIdx.x] = hist[e];
   }
 }
 
 // One block per block of k_route, the same rows.
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArgs a) {
   __shared__ int32_t before[kMaxExperts], all[kMaxExperts], at[kMaxExperts], tmp[kWarps + 1];
+  __shared__ int16_t ids[kSub];
   extern __shared__ int32_t count[];
-  for (int e = threadIdx.x; e < a.E; e += kThreads) before[e] = all[e] = 0;
-  __syncthreads();
   pdl_wait();
-  // kThreads / E threads share an expert's column of the blocks' counts.
-  const int share = kThreads / a.E, e = threadIdx.x % a.E, part = threadIdx.x / a.E;
-  if (part < share) {
-    int32_t b = 0, n = 0;
-#pragma unroll 16
-    for (int i = part; i < (int)gridDim.x; i += share) {
-      const int32_t v = a.hist[(int64_t)i * a.E + e];
-      n += v;
-      if (i < (int)blockIdx.x) b += v;
-    }
-    atomicAdd(&before[e], b);
-    atomicAdd(&all[e], n);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
+  const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
+  const int64_t p0 = r0 * a.k, p1 = r0 < r1 ? r1 * a.k : p0;
+  // The first pairs' experts are asked for before the counts, and stored after them.
+  int32_t first[kSub / kThreads];
+#pragma unroll
+  for (int i = 0; i < kSub / kThreads; i++) {
+    const int64_t p = p0 + i * kThreads + threadIdx.x;
+    first[i] = p < p1 ? a.experts[p] : -1;
   }
+  // A warp sums an expert's choices in all blocks and in those before this one.
+  for (int e = warp; e < a.E; e += kWarps) {
+    int32_t b = 0, n = 0;
+    const int32_t* row = a.hist + (int64_t)e * blocks;
+#pragma unroll 10
+    for (int i = lane; i < blocks; i += 32) {
+      const int32_t v = row[i];
+      n += v;
+      b += i < (int)blockIdx.x ? v : 0;
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    b = __reduce_add_sync(0xffffffffu, b);
+    if (lane == 0) {
+      all[e] = n;
+      before[e] = b;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kSub / kThreads; i++) ids[i * kThreads + threadIdx.x] = (int16_t)first[i];
   __syncthreads();
   const int32_t total = scan_experts(all, at, a.E, tmp);
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.E; i += kThreads) a.offsets[i] = at[i];
     if (threadIdx.x == 0) a.offsets[a.E] = total;
   }
+  __syncthreads();
   for (int i = threadIdx.x; i < a.E; i += kThreads) at[i] += before[i];
   __syncthreads();
-  const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
-  if (r0 < r1) assign_slots(a, r0 * a.k, r1 * a.k, at, count);
+  for (int64_t p = p0; p < p1; p += kSub) {
+    const int n = (int)(p1 - p < kSub ? p1 - p : kSub);
+    if (p > p0) {
+      __syncthreads();  // the last run's ids and counts have been read
+      for (int i = threadIdx.x; i < n; i += kThreads) ids[i] = (int16_t)a.experts[p + i];
+      __syncthreads();
+    }
+    assign_slots(a, p, n, ids, at, count);
+  }
 }
 
 constexpr int64_t kOneBlockPairs = 2048;
+static_assert(kOneBlockPairs <= kSub, "one block's pairs");
 
-template <typename T, int G>
-int32_t route_g(Ctx* c, const RouteArgs& a, int blocks) {
+template <typename T, int L, int KM>
+int32_t route_l(Ctx* c, const RouteArgs& a, int blocks) {
   const size_t smem = (size_t)kWarps * a.E * 4;  // at most 16 KB
   if (blocks == 1) {
-    FL_CUDA(c, launch_pdl(k_route<T, G, true>, dim3(1), dim3(kThreads), smem, c->stream, a));
+    FL_CUDA(c, launch_pdl(k_route<T, L, KM, true>, dim3(1), dim3(kThreads), smem + kSub * 2, c->stream, a));
     FL_LAUNCH(c);
     return FLETCHER_OK;
   }
-  FL_CUDA(c, launch_pdl(k_route<T, G, false>, dim3(blocks), dim3(kThreads), 0, c->stream, a));
+  FL_CUDA(c, launch_pdl(k_route<T, L, KM, false>, dim3(blocks), dim3(kThreads), 0, c->stream, a));
   FL_LAUNCH(c);
   FL_CUDA(c, launch_pdl(k_group, dim3(blocks), dim3(kThreads), smem, c->stream, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
 }
 
+template <typename T, int L>
+int32_t route_k(Ctx* c, const RouteArgs& a, int blocks) {
+  if (a.k <= 2) return route_l<T, L, 2>(c, a, blocks);
+  if (a.k <= 8) return route_l<T, L, 8>(c, a, blocks);
+  return route_l<T, L, 16>(c, a, blocks);
+}
+
+// Lanes a row: one where a chunk holds all experts; a warp for few rows of many.
+int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E <= 4 * V || a.rows > 2048 ? 4 : 32; }
+
 template <typename T>
 int32_t route_t(Ctx* c, const RouteArgs& a, int blocks) {
-  const int lanes = (a.E + V - 1) / V;
-  if (lanes <= 1) return route_g<T, 1>(c, a, blocks);
-  if (lanes <= 2) return route_g<T, 2>(c, a, blocks);
-  if (lanes <= 4) return route_g<T, 4>(c, a, blocks);
-  if (lanes <= 8) return route_g<T, 8>(c, a, blocks);
-  if (lanes <= 16) return route_g<T, 16>(c, a, blocks);
-  return route_g<T, 32>(c, a, blocks);
+  const int lanes = lanes_of(a);
+  return lanes == 1 ? route_k<T, 1>(c, a, blocks) : lanes == 4 ? route_k<T, 4>(c, a, blocks) : route_k<T, 32>(c, a, blocks);
 }
 
 int max_blocks(const Ctx* c) { return kBlocksPerSM * c->num_sms; }
@@ -359,8 +457,13 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   const int64_t pairs = a.rows * a.k;
   // A block for every 256 pairs, to keep short batches wide, up to two blocks an SM.
   const int64_t want = pairs <= kOneBlockPairs ? 1 : (pairs + 255) / 256;
-  const int blocks = (int)std::min<int64_t>(want, max_blocks(c));
+  int blocks = (int)std::min<int64_t>(want, max_blocks(c));
   a.chunk = (a.rows + blocks - 1) / blocks;
+  if (blocks > 1) {  // whole passes of a block's threads
+    const int64_t pass = kThreads / lanes_of(a);
+    a.chunk = (a.chunk + pass - 1) / pass * pass;
+    blocks = (int)((a.rows + a.chunk - 1) / a.chunk);
+  }
   if (dtype == FLETCHER_BF16) return route_t<__nv_bfloat16>(c, a, blocks);
   if (dtype == FLETCHER_F16) return route_t<__half>(c, a, blocks);
   return route_t<float>(c, a, blocks);
