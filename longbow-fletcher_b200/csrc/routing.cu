@@ -10,11 +10,12 @@
 // issue: L = 4 lanes a row for many rows (65536 x 64 -> 6: 82 instructions a row, against 164 with 8
 // lanes that hold eight keys each), a whole warp a row where rows are few and latency counts.
 //
-// Grouping is a stable counting sort in two launches without atomics on memory: k_route leaves, per
-// block of rows, how many choices each expert got; k_group sums the blocks before its own (and all
-// of them, for the offsets), ranks its pairs within the block, and writes slots and their inverse.
-// Up to kOneBlockPairs pairs one block does both in one launch.  Nothing depends on the order in
-// which blocks or atomics run, so the slots are the same in every run.
+// Grouping is a stable counting sort in two launches: k_route leaves, per block of rows, how many
+// choices each expert got, and its last block to finish turns these into what precedes each block;
+// k_group ranks its pairs within the block and writes slots and their inverse.  (Summed by every
+// block of k_group instead, the same lines of L2 are read by all at once: 9 of 19 us.)  Up to
+// kOneBlockPairs pairs one block does all in one launch.  Which block is last changes nothing in the
+// result, so the slots are the same in every run.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -27,31 +28,46 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBlocksPerSM = 2;
 constexpr int V = 8;  // logits per lane
-// Keys.  0 for what is never chosen: -inf and NaN; +0 and -0 are equal.
+// Keys of eight logits from expert e0 on, and the logits in fp32.  NaN counts as -inf and -0 as +0;
+// a key that is not `valid` (-inf, or the 0 of an empty place) is never chosen.
 template <typename T>
 struct KeyOf {  // f32
   typedef unsigned long long K;
-  static __device__ __forceinline__ K make(float x, int e) {
-    if (!(x > -INFINITY)) return 0;
-    if (x == 0.0f) x = 0.0f;
-    const uint32_t b = __float_as_uint(x);
-    return ((K)((b & 0x80000000u) ? ~b : b | 0x80000000u) << 32) | (uint32_t)~e;
+  static __device__ __forceinline__ void make(const float (&t)[V], int e0, K (&key)[V], float (&x)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      x[i] = fmaxf(t[i], -INFINITY) + 0.0f;
+      const uint32_t b = __float_as_uint(x[i]);
+      key[i] = ((K)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32) | (uint32_t)~(e0 + i);
+    }
   }
+  static __device__ __forceinline__ bool valid(K k) { return (uint32_t)(k >> 32) > 0x007fffffu; }
   static __device__ __forceinline__ int expert(K k) { return (int)~(uint32_t)k; }
   static __device__ __forceinline__ float value(K k) {
     const uint32_t o = (uint32_t)(k >> 32);
     return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
   }
 };
-template <typename T>
+template <typename T, typename T2, uint32_t NEG_INF>
 struct KeyOf16 {
   typedef uint32_t K;
-  static __device__ __forceinline__ K make(T x, int e) {
-    const float f = to_f<T>(x);
-    if (!(f > -INFINITY)) return 0;
-    const uint32_t b = f == 0.0f ? 0 : *reinterpret_cast<const uint16_t*>(&x);
-    return (((b & 0x8000u) ? ~b & 0xffffu : b | 0x8000u) << 16) | (uint32_t)(0xffff - e);
+  // Two logits a word: the maximum with -inf drops NaN, adding +0 turns -0 over, and flipping a negative
+  // number's bits, a positive one's sign, orders both halves.
+  static __device__ __forceinline__ void make(const T (&t)[V], int e0, K (&key)[V], float (&x)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const uint32_t inf2 = NEG_INF * 0x10001u, zero2 = 0;
+      const T2 v = __hadd2(__hmax2(*reinterpret_cast<const T2*>(&t[i]), *reinterpret_cast<const T2*>(&inf2)),
+                           *reinterpret_cast<const T2*>(&zero2));
+      uint32_t u = *reinterpret_cast<const uint32_t*>(&v);
+      x[i] = to_f<T>(v.x);
+      x[i + 1] = to_f<T>(v.y);
+      u ^= ((u >> 15) & 0x10001u) * 0xffffu | 0x80008000u;
+      key[i] = (u << 16) | (uint32_t)(0xffff - e0 - i);
+      key[i + 1] = (u & 0xffff0000u) | (uint32_t)(0xffff - e0 - i - 1);
+    }
   }
+  static __device__ __forceinline__ bool valid(K k) { return k >> 16 > (NEG_INF ^ 0xffffu); }
   static __device__ __forceinline__ int expert(K k) { return 0xffff - (int)(k & 0xffffu); }
   static __device__ __forceinline__ float value(K k) {
     const uint32_t o = k >> 16;
@@ -60,9 +76,9 @@ struct KeyOf16 {
   }
 };
 template <>
-struct KeyOf<__half> : KeyOf16<__half> {};
+struct KeyOf<__half> : KeyOf16<__half, __half2, 0xfc00u> {};
 template <>
-struct KeyOf<__nv_bfloat16> : KeyOf16<__nv_bfloat16> {};
+struct KeyOf<__nv_bfloat16> : KeyOf16<__nv_bfloat16, __nv_bfloat162, 0xff80u> {};
 
 // Eight keys in descending order.
 template <typename K>
@@ -94,18 +110,20 @@ struct RouteArgs {
   int32_t* slots;
   int32_t* pair_of;
   int32_t* offsets;
-  int32_t* hist;
+  int32_t* hist;    // [E, stride]
+  int32_t* ticket;  // blocks of k_route that have finished; 0 between launches
+  int32_t stride;
 };
 
-// exp(x - m) on the special-function unit, where x may equal an infinite m: the difference is rounded
-// once, its product with log2 e once more, so the relative error is about (|x - m| + 3) * 2^-24, and terms
-// far below the maximum, where that grows, are small.
-__device__ __forceinline__ float exp_below(float x, float m) {
-  const float t = x == m ? 0.0f : x - m;
+// e^d on the special-function unit: d's product with log2 e is rounded once, so the relative error is
+// about (|d| + 2) * 2^-24; terms far below the maximum, where that grows, are small.
+__device__ __forceinline__ float exp_fast2(float d) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t * 1.44269504f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.44269504f));
   return y;
 }
+// exp(x - m) where x may equal an infinite m.
+__device__ __forceinline__ float exp_below(float x, float m) { return x == m ? 1.0f : exp_fast2(x - m); }
 
 // The choices and weights of rows [r0, r1), into `hist` (shared) each expert's count, and, unless null,
 // the choices into `ids` (shared).
@@ -119,22 +137,20 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
   const int chunks = (a.E + V * L - 1) / (V * L);
   const T* z = reinterpret_cast<const T*>(a.logits);
   const bool vec = a.E % V == 0 && ((uintptr_t)z & 15) == 0;
-  union Chunk {
-    uint4 q[sizeof(T) * V / 16];
+  struct alignas(16) Chunk {
     T t[V];
   };
-  // Whole teams step together; a team past the end works on the last row and writes nothing.
+  // Whole teams step together; a team past the end works on the last row and writes nothing.  Places past
+  // the experts are -inf.
   auto load = [&](int64_t r, int e0, Chunk& u) {
     const T* row = z + (r < r1 ? r : r1 - 1) * a.E + e0;
-    if (vec) {
-      if (e0 < a.E) {
+    if (vec && e0 < a.E) {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) * V / 16); i++) u.q[i] = __ldg(reinterpret_cast<const uint4*>(row) + i);
-      }
+      for (int i = 0; i < (int)sizeof(Chunk) / 16; i++)
+        reinterpret_cast<uint4*>(&u)[i] = __ldg(reinterpret_cast<const uint4*>(row) + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        if (e0 + i < a.E) u.t[i] = row[i];
+      for (int i = 0; i < V; i++) u.t[i] = e0 + i < a.E ? row[i] : from_f<T>(-INFINITY);
     }
   };
   const bool all = !a.sigmoid && !a.normalise;  // the weights' sum is over the whole row
@@ -143,7 +159,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
   for (int64_t base = r0; base < r1; base += kPass) {
     const int64_t mine = base + threadIdx.x / L;
     K list[KM] = {};
-    float lane_max = -INFINITY, lane_sum = 0.f;
+    float ref = 0.f, sum = 0.f, top = -INFINITY;  // sum of exp(x - ref) over the lane's logits, their maximum
     for (int c = 0; c < chunks; c++) {
       const int e0 = (c * L + gl) * V;
       const Chunk cur = next;
@@ -152,20 +168,21 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
       else if (base + kPass < r1)
         load(mine + kPass, gl * V, next);
       K key[V];
+      float x[V];
+      Key::make(cur.t, e0, key, x);
+      if (all) {
 #pragma unroll
-      for (int i = 0; i < V; i++) key[i] = e0 + i < a.E ? Key::make(cur.t[i], e0 + i) : 0;
-      if (all) {  // running maximum and sum
-        float x[V], mx = lane_max;
+        for (int i = 0; i < V; i++) top = fmaxf(top, x[i]);
+        const float r = fabsf(top) == INFINITY ? 0.f : top;  // +inf is counted below instead
+        sum = sum > 0.f ? sum * exp_fast2(ref - r) : 0.f;
+        ref = r;
+        float s1 = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          x[i] = key[i] ? to_f<T>(cur.t[i]) : -INFINITY;
-          mx = fmaxf(mx, x[i]);
+        for (int i = 0; i < V; i += 2) {
+          add2(x[i], x[i + 1], -r, -r);
+          add2(sum, s1, exp_fast2(x[i]), exp_fast2(x[i + 1]));
         }
-        lane_sum *= exp_below(lane_max, mx);
-        lane_max = mx;
-#pragma unroll
-        for (int i = 0; i < V; i++)
-          if (key[i]) lane_sum += exp_below(x[i], mx);
+        sum += s1;
       }
       if (KM >= V && c == 0) {
         sort8(key);
@@ -200,7 +217,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
             const K other = __shfl_xor_sync(0xffffffffu, best, o);
             best = other > best ? other : best;
           }
-          const bool own = list[0] == best;  // keys are unique: one lane (or, at 0, lanes with nothing left)
+          const bool own = list[0] == best;  // keys are unique: one lane (or, at 0, all with nothing left)
 #pragma unroll
           for (int i = 0; i < KM; i++) list[i] = own ? (i + 1 < KM ? list[i + 1] : 0) : list[i];
           if (j == 0) m = Key::value(best);
@@ -212,13 +229,20 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
 #pragma unroll
     for (int j = 0; j < KEEP; j++) {
       w[j] = 0.f;
-      if (kept[j]) {
+      if (Key::valid(kept[j])) {
         const float v = Key::value(kept[j]);
         w[j] = a.sigmoid ? 1.0f / (1.0f + expf(-v)) : exp_below(v, m);
       }
       total += w[j];
     }
-    if (all) total = lane_sum * exp_below(lane_max, m);
+    if (all) {
+      total = sum > 0.f ? sum * exp_fast2(ref - m) : 0.f;
+      if (m == INFINITY) {  // the row's +inf share the weight
+        total = 0.f;
+        for (int e = gl; e < a.E; e += L)
+          total += to_f<T>(z[(mine < r1 ? mine : r1 - 1) * a.E + e]) == INFINITY ? 1.f : 0.f;
+      }
+    }
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     // Divided by the sum first, so that no product overflows before it; 0 where the sum is 0.
@@ -229,7 +253,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
       for (int i = 0; i < KEEP; i++) {
         const int j = i * L + gl;
         if (j < a.k) {
-          const int id = kept[i] ? Key::expert(kept[i]) : -1;
+          const int id = Key::valid(kept[i]) ? Key::expert(kept[i]) : -1;
           a.experts[out + j] = id;
           a.weights[out + j] = w[i] * inv * a.scale;
           if (ids) ids[(int)(out - r0 * a.k) + j] = (int16_t)id;
@@ -349,61 +373,63 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
     if (threadIdx.x == 0) a.offsets[a.E] = total;
     assign_slots(a, 0, (int)(r1 * a.k), ids, at, dyn);
   } else {
-    for (int e = threadIdx.x; e < a.E; e += kThreads) a.hist[(int64_t)e * gridDim.x + blockIdx.x] = hist[e];
+    for (int e = threadIdx.x; e < a.E; e += kThreads) a.hist[(int64_t)e * a.stride + blockIdx.x] = hist[e];
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    __shared__ int32_t at[kMaxExperts], tmp[kWarps + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
+    if (threadIdx.x == 0) *a.ticket = 0;
+    // A warp an expert: counts become exclusive sums over the blocks, four a lane.
+    for (int e = warp; e < a.E; e += kWarps) {
+      int4* row = reinterpret_cast<int4*>(a.hist + (int64_t)e * a.stride);
+      int32_t carry = 0;
+#pragma unroll 4
+      for (int i = lane; i - lane < (blocks + 3) / 4; i += 32) {
+        int4 v = 4 * i < blocks ? __ldcg(row + i) : make_int4(0, 0, 0, 0);
+        if (4 * i + 1 >= blocks) v.y = 0;
+        if (4 * i + 2 >= blocks) v.z = 0;
+        if (4 * i + 3 >= blocks) v.w = 0;
+        const int32_t n = v.x + v.y + v.z + v.w;
+        int32_t s = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += u;
+        }
+        const int32_t b = carry + s - n;
+        if (4 * i < blocks) row[i] = make_int4(b, b + v.x, b + v.x + v.y, b + v.x + v.y + v.z);
+        carry += __shfl_sync(0xffffffffu, s, 31);
+      }
+      if (lane == 0) hist[e] = carry;
+    }
+    __syncthreads();
+    const int32_t total = scan_experts(hist, at, a.E, tmp);
+    for (int e = threadIdx.x; e < a.E; e += kThreads) a.offsets[e] = at[e];
+    if (threadIdx.x == 0) a.offsets[a.E] = total;
   }
 }
 
 // One block per block of k_route, the same rows.
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArgs a) {
-  __shared__ int32_t before[kMaxExperts], all[kMaxExperts], at[kMaxExperts], tmp[kWarps + 1];
+  __shared__ int32_t at[kMaxExperts];
   __shared__ int16_t ids[kSub];
   extern __shared__ int32_t count[];
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
   const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
   const int64_t p0 = r0 * a.k, p1 = r0 < r1 ? r1 * a.k : p0;
-  // The first pairs' experts are asked for before the counts, and stored after them.
-  int32_t first[kSub / kThreads];
-#pragma unroll
-  for (int i = 0; i < kSub / kThreads; i++) {
-    const int64_t p = p0 + i * kThreads + threadIdx.x;
-    first[i] = p < p1 ? a.experts[p] : -1;
-  }
-  // A warp sums an expert's choices in all blocks and in those before this one.
-  for (int e = warp; e < a.E; e += kWarps) {
-    int32_t b = 0, n = 0;
-    const int32_t* row = a.hist + (int64_t)e * blocks;
-#pragma unroll 10
-    for (int i = lane; i < blocks; i += 32) {
-      const int32_t v = row[i];
-      n += v;
-      b += i < (int)blockIdx.x ? v : 0;
-    }
-    n = __reduce_add_sync(0xffffffffu, n);
-    b = __reduce_add_sync(0xffffffffu, b);
-    if (lane == 0) {
-      all[e] = n;
-      before[e] = b;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kSub / kThreads; i++) ids[i * kThreads + threadIdx.x] = (int16_t)first[i];
-  __syncthreads();
-  const int32_t total = scan_experts(all, at, a.E, tmp);
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < a.E; i += kThreads) a.offsets[i] = at[i];
-    if (threadIdx.x == 0) a.offsets[a.E] = total;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.E; i += kThreads) at[i] += before[i];
-  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += kThreads) at[e] = a.offsets[e] + a.hist[(int64_t)e * a.stride + blockIdx.x];
   for (int64_t p = p0; p < p1; p += kSub) {
     const int n = (int)(p1 - p < kSub ? p1 - p : kSub);
-    if (p > p0) {
-      __syncthreads();  // the last run's ids and counts have been read
-      for (int i = threadIdx.x; i < n; i += kThreads) ids[i] = (int16_t)a.experts[p + i];
-      __syncthreads();
-    }
+    __syncthreads();  // the last run's ids and counts have been read
+#pragma unroll
+    for (int i = 0; i < kSub; i += kThreads)
+      if (i + (int)threadIdx.x < n) ids[i + threadIdx.x] = (int16_t)a.experts[p + i + threadIdx.x];
+    __syncthreads();
     assign_slots(a, p, n, ids, at, count);
   }
 }
@@ -434,7 +460,7 @@ int32_t route_k(Ctx* c, const RouteArgs& a, int blocks) {
 }
 
 // Lanes a row: one where a chunk holds all experts; a warp for few rows of many.
-int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E <= 4 * V || a.rows > 2048 ? 4 : 32; }
+int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E <= 4 * V || a.rows > 2 * kThreads / 32 ? 4 : 32; }
 
 template <typename T>
 int32_t route_t(Ctx* c, const RouteArgs& a, int blocks) {
@@ -442,7 +468,7 @@ int32_t route_t(Ctx* c, const RouteArgs& a, int blocks) {
   return lanes == 1 ? route_k<T, 1>(c, a, blocks) : lanes == 4 ? route_k<T, 4>(c, a, blocks) : route_k<T, 32>(c, a, blocks);
 }
 
-int max_blocks(const Ctx* c) { return kBlocksPerSM * c->num_sms; }
+int max_blocks(const Ctx* c) { return kBlocksPerSM * c->num_sms / 4 * 4; }  // rows of int4
 
 int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   Ctx* c = r->c;
@@ -454,6 +480,8 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   a.pair_of = r->pair_of;
   a.offsets = r->offsets;
   a.hist = r->hist;
+  a.ticket = r->ticket;
+  a.stride = max_blocks(c);
   const int64_t pairs = a.rows * a.k;
   // A block for every 256 pairs, to keep short batches wide, up to two blocks an SM.
   const int64_t want = pairs <= kOneBlockPairs ? 1 : (pairs + 255) / 256;
@@ -522,7 +550,7 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
   r->num_experts = num_experts;
   r->top_k = top_k;
   const int64_t pairs = (max_rows * top_k + 3) / 4 * 4;  // keeps every array 16-byte aligned
-  const int64_t ints = 4 * pairs + (num_experts + 1 + 3) / 4 * 4 + (int64_t)max_blocks(c) * num_experts;
+  const int64_t ints = 4 * pairs + (num_experts + 1 + 3) / 4 * 4 + (int64_t)max_blocks(c) * num_experts + 4;
   r->bytes = ints * 4;
   const int32_t rc = dev_alloc(c, &r->mem, r->bytes);
   if (rc) {
@@ -535,6 +563,7 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
   r->pair_of = r->experts + 3 * pairs;
   r->offsets = r->experts + 4 * pairs;
   r->hist = r->offsets + (num_experts + 1 + 3) / 4 * 4;
+  r->ticket = r->hist + (int64_t)max_blocks(c) * num_experts;  // 0, as dev_alloc fills
   *out = r;
   return FLETCHER_OK;
 }
