@@ -7,9 +7,6 @@
 namespace fl {
 namespace {
 
-constexpr int BM = 64, BN = 64, BK = 16, TM = 4, TN = 4;
-constexpr int kThreads = (BM / TM) * (BN / TN);
-
 // The block's group and rows: m-tile `tile` of all groups' m-tiles in order; the tile's first slot
 // and the group's end, expert -1 when there are fewer tiles.  Called by one warp.
 __device__ __forceinline__ void find_tile(const int32_t* __restrict__ offsets, int E, int tile, int rows_per_tile,
@@ -51,60 +48,119 @@ __device__ __forceinline__ float act1(float v) {
   return v;
 }
 
-// One 64 x 64 output tile a block (SwiGLU: its gate and up columns), 4 x 4 sums a thread, K in
-// slabs of 16 through shared memory; rows are gathered as the slab is loaded.
-template <typename T, int ACT>
-__global__ void __launch_bounds__(kThreads) k_grouped_simt(const GroupedArgs a) {
+// One BM x BN output tile a block (SwiGLU: its gate and up columns), TM x TN sums a thread in packed pairs
+// along n, K in slabs of 16: the next slab's elements are on their way from memory while this one's are
+// multiplied from shared memory.  Rows are gathered as they are loaded; single elements, so that any
+// width and alignment does.  KS teams of threads take alternate slabs.  Bound by the fp32 units (34
+// TFLOP/s at 4000 x 2 rows of 8 experts, 500 -> 500), for few rows by a slab's chain of load, store and
+// multiply, which teams overlap.
+template <typename T, int ACT, int BM, int BN, int TM, int TN, int KS>
+__global__ void __launch_bounds__((BM / TM) * (BN / TN) * KS) k_grouped_simt(const GroupedArgs a) {
+  constexpr int BK = 16, kThreads = (BM / TM) * (BN / TN);  // of one of the KS teams
   constexpr bool GATED = ACT == FLETCHER_ACT_SWIGLU;
   constexpr int NB = GATED ? 2 : 1;
-  __shared__ float sx[BK][BM + 4], sw[NB][BK][BN];
+  constexpr int XL = BM * BK / kThreads, WL = BN * BK / kThreads;  // elements a thread loads
+  static_assert(kThreads % BK == 0 && kThreads % BN == 0 && TM % 4 == 0 && TN == 4, "thread layout");
+  __shared__ __align__(16) float s_x[KS][2][BK][BM + 4], s_w[KS][2][NB][BK][BN];
   __shared__ int32_t s_tile[3];
-  __shared__ int64_t s_row[BM];
+  const int tid = threadIdx.x % kThreads, team = threadIdx.x / kThreads;
+  auto& sx = s_x[team];
+  auto& sw = s_w[team];
+  auto team_sync = [&]() {
+    if constexpr (KS > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kThreads) : "memory");
+    else
+      __syncthreads();
+  };
   const unsigned nt = (unsigned)((a.n_out + BN - 1) / BN);  // n-tiles, fastest
   pdl_wait();
   if (threadIdx.x < 32) find_tile(a.offsets, a.experts, (int)(blockIdx.x / nt), BM, &s_tile[0], &s_tile[1], &s_tile[2]);
   __syncthreads();
   const int e = s_tile[0];
   if (e < 0) return;
-  const int64_t first = s_tile[1], end = s_tile[2];
-  for (int i = threadIdx.x; i < BM; i += kThreads) {
-    const int64_t s = first + i;
-    s_row[i] = s >= end ? -1 : a.pair_of ? a.pair_of[s] / a.top_k : s;
-  }
-  __syncthreads();
+  const int first = s_tile[1], end = s_tile[2];
   const int64_t n0 = (int64_t)(blockIdx.x % nt) * BN;
-  const T* x = reinterpret_cast<const T*>(a.x);
-  const T* w = reinterpret_cast<const T*>(a.w) + (int64_t)e * a.K * a.N;
-  const int tx = threadIdx.x % (BN / TN), ty = threadIdx.x / (BN / TN);
-  float acc[NB][TM][TN] = {};
-  for (int64_t k0 = 0; k0 < a.K; k0 += BK) {
-    for (int i = threadIdx.x; i < BM * BK; i += kThreads) {
-      const int m = i / BK, k = i % BK;
-      const int64_t r = s_row[m];
-      sx[k][m] = r >= 0 && k0 + k < a.K ? to_f<T>(x[r * a.K + k0 + k]) : 0.f;
-    }
+  // This thread loads column xk of rows xm + i * (kThreads / BK), and column wn of rows wk + i * (kThreads / BN).
+  const int xk = tid % BK, xm = tid / BK, wn = tid % BN, wk = tid / BN;
+  const T* xrow[XL];
+#pragma unroll
+  for (int i = 0; i < XL; i++) {
+    const int s = first + xm + i * (kThreads / BK);
+    const int64_t r = s >= end ? -1 : a.pair_of ? a.pair_of[s] / a.top_k : s;
+    xrow[i] = r < 0 ? nullptr : reinterpret_cast<const T*>(a.x) + r * a.K + xk;
+  }
+  const T* w = reinterpret_cast<const T*>(a.w) + (int64_t)e * a.K * a.N + n0 + wn;
+  const bool w_in = n0 + wn < a.n_out;
+  T rx[XL], rw[NB][WL];
+  auto load = [&](int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < XL; i++) rx[i] = xrow[i] && k0 + xk < a.K ? xrow[i][k0] : from_f<T>(0.f);
 #pragma unroll
     for (int b = 0; b < NB; b++)
-      for (int i = threadIdx.x; i < BK * BN; i += kThreads) {
-        const int k = i / BN, n = i % BN;
-        sw[b][k][n] = k0 + k < a.K && n0 + n < a.n_out ? to_f<T>(w[(k0 + k) * a.N + b * a.n_out + n0 + n]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < WL; i++) {
+        const int64_t k = k0 + wk + i * (kThreads / BN);
+        rw[b][i] = w_in && k < a.K ? w[k * a.N + b * a.n_out] : from_f<T>(0.f);
       }
-    __syncthreads();
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < XL; i++) sx[buf][xk][xm + i * (kThreads / BK)] = to_f<T>(rx[i]);
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < WL; i++) sw[buf][b][wk + i * (kThreads / BN)][wn] = to_f<T>(rw[b][i]);
+  };
+  const int tx = tid % (BN / TN), ty = tid / (BN / TN);
+  float acc[NB][TM][TN] = {};
+  load(team * BK);
+  store(0);
+  team_sync();
+  int buf = 0;
+  for (int64_t k0 = team * BK; k0 < a.K; k0 += KS * BK, buf ^= 1) {
+    const bool more = k0 + KS * BK < a.K;
+    if (more) load(k0 + KS * BK);
 #pragma unroll
     for (int k = 0; k < BK; k++) {
       float xv[TM];
 #pragma unroll
-      for (int i = 0; i < TM; i++) xv[i] = sx[k][ty * TM + i];
+      for (int i = 0; i < TM; i += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(&sx[buf][k][ty * TM + i]);
+        xv[i] = q.x, xv[i + 1] = q.y, xv[i + 2] = q.z, xv[i + 3] = q.w;
+      }
 #pragma unroll
-      for (int b = 0; b < NB; b++)
+      for (int b = 0; b < NB; b++) {
+        const float4 q = *reinterpret_cast<const float4*>(&sw[buf][b][k][tx * TN]);
 #pragma unroll
-        for (int j = 0; j < TN; j++) {
-          const float wv = sw[b][k][tx * TN + j];
-#pragma unroll
-          for (int i = 0; i < TM; i++) acc[b][i][j] = fmaf(xv[i], wv, acc[b][i][j]);
+        for (int i = 0; i < TM; i++) {
+          float* c = acc[b][i];
+          fma2(c[0], c[1], xv[i], xv[i], q.x, q.y, c[0], c[1]);
+          fma2(c[2], c[3], xv[i], xv[i], q.z, q.w, c[2], c[3]);
         }
+      }
     }
-    __syncthreads();
+    if (more) store(buf ^ 1);
+    team_sync();
+  }
+  if constexpr (KS > 1) {  // the teams' sums, added in their order by the first
+    float* red = &s_x[0][0][0][0];
+    static_assert(sizeof(s_x) >= sizeof(float) * (KS - 1) * kThreads * TM * TN, "room for one operand's sums");
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      __syncthreads();
+      if (team > 0) {
+#pragma unroll
+        for (int i = 0; i < TM * TN; i++) red[((team - 1) * TM * TN + i) * kThreads + tid] = acc[b][i / TN][i % TN];
+      }
+      __syncthreads();
+      if (team == 0) {
+#pragma unroll
+        for (int t = 0; t < KS - 1; t++)
+#pragma unroll
+          for (int i = 0; i < TM * TN; i++) acc[b][i / TN][i % TN] += red[(t * TM * TN + i) * kThreads + tid];
+      }
+    }
+    if (team > 0) return;
   }
   const T* bias = a.bias ? reinterpret_cast<const T*>(a.bias) + (int64_t)e * a.N : nullptr;
   T* out = reinterpret_cast<T*>(a.out);
@@ -118,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) k_grouped_simt(const GroupedArgs a) 
       if (n >= a.n_out) continue;
       float v = acc[0][i][j] + (bias ? to_f<T>(bias[n]) : 0.f);
       if constexpr (GATED) {
-        const float u = acc[1][i][j] + (bias ? to_f<T>(bias[a.n_out + n]) : 0.f);
+        const float u = acc[NB - 1][i][j] + (bias ? to_f<T>(bias[a.n_out + n]) : 0.f);
         v = sizeof(T) == 4 ? swiglu_exact(v, u) : __fdividef(v, 1.0f + __expf(-v)) * u;
       } else {
         v = act1<T, ACT>(v);
@@ -128,28 +184,39 @@ __global__ void __launch_bounds__(kThreads) k_grouped_simt(const GroupedArgs a) 
   }
 }
 
-template <typename T>
-int32_t launch(Ctx* c, const GroupedArgs& a) {
+template <typename T, int ACT, int BM, int BN, int TM, int TN, int KS>
+int32_t run(Ctx* c, const GroupedArgs& a) {
   const int64_t nt = (a.n_out + BN - 1) / BN;
-  const int64_t mt = (a.pairs + BM - 1) / BM + std::min<int64_t>(a.experts, a.pairs);  // at most this many m-tiles
+  const int64_t mt = a.pairs / BM + std::min<int64_t>(a.experts, a.pairs);  // at most this many m-tiles
   FL_CHECK(c, nt * mt <= INT32_MAX, "Linear_Grouped: %lldx%lld is too large for the fp32 units", (long long)a.pairs,
            (long long)a.n_out);
-  const dim3 grid((unsigned)(nt * mt));
-#define FL_ACT(A)                                                                                      \
-  case A:                                                                                              \
-    FL_CUDA(c, launch_pdl(k_grouped_simt<T, A>, grid, dim3(kThreads), 0, c->stream, a));               \
-    break
-  switch (a.act) {
-    FL_ACT(FLETCHER_ACT_IDENTITY);
-    FL_ACT(FLETCHER_ACT_GELU);
-    FL_ACT(FLETCHER_ACT_TANH);
-    FL_ACT(FLETCHER_ACT_SWIGLU);
-    default:
-      return set_error(c, FLETCHER_ERR_INVALID, "Linear_Grouped: unknown activation %d", a.act);
-  }
-#undef FL_ACT
+  FL_CUDA(c, launch_pdl(k_grouped_simt<T, ACT, BM, BN, TM, TN, KS>, dim3((unsigned)(nt * mt)),
+                        dim3((BM / TM) * (BN / TN) * KS), 0, c->stream, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
+}
+
+template <typename T, int ACT>
+int32_t pick(Ctx* c, const GroupedArgs& a) {
+  // 64 x 64 tiles where there are two for every SM, else 32 x 32 by four teams (SwiGLU's two operands: two),
+  // so that more SMs and warps share few rows (509 rows of 5 experts, 129 -> 130: 8.6 us, 15.1 in 64 x 64 tiles).
+  const int64_t tiles = (a.pairs / 64 + std::min<int64_t>(a.experts, a.pairs)) * ((a.n_out + 63) / 64);
+  if (tiles >= 2 * c->num_sms) return run<T, ACT, 64, 64, 8, 4, 1>(c, a);
+  return run<T, ACT, 32, 32, 4, 4, ACT == FLETCHER_ACT_SWIGLU ? 2 : 4>(c, a);
+}
+
+template <typename T>
+int32_t launch(Ctx* c, const GroupedArgs& a) {
+  switch (a.act) {
+    case FLETCHER_ACT_IDENTITY:
+      return pick<T, FLETCHER_ACT_IDENTITY>(c, a);
+    case FLETCHER_ACT_GELU:
+      return pick<T, FLETCHER_ACT_GELU>(c, a);
+    case FLETCHER_ACT_TANH:
+      return pick<T, FLETCHER_ACT_TANH>(c, a);
+    default:
+      return pick<T, FLETCHER_ACT_SWIGLU>(c, a);
+  }
 }
 
 }  // namespace
