@@ -36,11 +36,49 @@ struct NormArgs {
   int32_t cols;
 };
 
-template <typename T>
-union Pack {
-  uint4 q;
-  T t[16 / sizeof(T)];
+// VEC elements moved at once: 16 bytes, or what a row's width and alignment allow.
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<16> {
+  typedef uint4 R;
 };
+template <>
+struct RawOf<4> {
+  typedef uint32_t R;
+};
+template <>
+struct RawOf<2> {
+  typedef uint16_t R;
+};
+template <typename T, int VEC>
+union Pack {
+  typename RawOf<VEC * sizeof(T)>::R q;
+  T t[VEC];
+};
+
+// One step of S = 2 values in packed fp32, or of one.
+template <int S>
+__device__ __forceinline__ void fma_s(float* d, const float* a, float b0, float b1, const float* c) {
+  if constexpr (S == 1)
+    d[0] = fmaf(a[0], b0, c[0]);
+  else
+    fma2(d[0], d[1], a[0], a[1], b0, b1, c[0], c[1]);
+}
+template <int S>
+__device__ __forceinline__ void mul_s(float* d, float b0, float b1) {
+  if constexpr (S == 1)
+    d[0] *= b0;
+  else
+    mul2(d[0], d[1], d[0], d[1], b0, b1);
+}
+template <int S>
+__device__ __forceinline__ void add_s(float* d, float b) {
+  if constexpr (S == 1)
+    d[0] += b;
+  else
+    add2(d[0], d[1], b, b);
+}
 
 // Sum over the team's lanes.  `red` has kSlots turns of 8 floats; turns alternate so that a warp
 // that is still reading one sum cannot meet the next sum's writes.
@@ -69,41 +107,52 @@ __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const f
   constexpr int TPR = 32 * WPR;
   if (kind == FLETCHER_NORM_NONE) return;
   // In packed pairs of fp32: half the instructions, which at 16-bit widths weigh as much as the bytes.
-  float s0 = 0.f, s1 = 0.f, mean = 0.f;
+  constexpr int S = VEC == 1 ? 1 : 2, Q = VEC < 4 ? S : 4;  // values a step, and a load of gamma or beta
+  float mean = 0.f;
   if (kind == FLETCHER_NORM_LAYER) {
+    float p[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NV * VEC; i += 2) add2(s0, s1, v[i], v[i + 1]);
-    mean = team_sum<WPR>(s0 + s1, red, turn) / (float)cols;
-    s0 = s1 = 0.f;
+    for (int i = 0; i < NV * VEC; i += 2) add2(p[0], p[1], v[i], v[i + 1]);
+    mean = team_sum<WPR>(p[0] + p[1], red, turn) / (float)cols;
   }
+  float q[2] = {0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < NV; j++) {
     if (j * TPR + t < nvec) {
 #pragma unroll
-      for (int i = j * VEC; i < (j + 1) * VEC; i += 2) {
-        if (kind == FLETCHER_NORM_LAYER) add2(v[i], v[i + 1], -mean, -mean);
-        fma2(s0, s1, v[i], v[i + 1], v[i], v[i + 1], s0, s1);
+      for (int i = j * VEC; i < (j + 1) * VEC; i += S) {
+        if (kind == FLETCHER_NORM_LAYER) add_s<S>(&v[i], -mean);
+        fma_s<S>(q, &v[i], v[i], S == 2 ? v[i + S - 1] : 0.f, q);
       }
     }
   }
-  const float inv = 1.0f / sqrtf(team_sum<WPR>(s0 + s1, red, turn) / (float)cols + eps);
+  const float inv = 1.0f / sqrtf(team_sum<WPR>(q[0] + q[1], red, turn) / (float)cols + eps);
 #pragma unroll
   for (int j = 0; j < NV; j++) {
     const int at = j * TPR + t;
     if (at < nvec) {
 #pragma unroll
-      for (int i = 0; i < VEC; i += 4) {
-        float* p = &v[j * VEC + i];
-        mul2(p[0], p[1], p[0], p[1], inv, inv);
-        mul2(p[2], p[3], p[2], p[3], inv, inv);
-        const float4 g = gamma ? __ldg(reinterpret_cast<const float4*>(gamma + at * VEC + i)) : make_float4(1.f, 1.f, 1.f, 1.f);
-        if (beta) {
-          const float4 b = __ldg(reinterpret_cast<const float4*>(beta + at * VEC + i));
-          fma2(p[0], p[1], p[0], p[1], g.x, g.y, b.x, b.y);
-          fma2(p[2], p[3], p[2], p[3], g.z, g.w, b.z, b.w);
-        } else {
-          mul2(p[0], p[1], p[0], p[1], g.x, g.y);
-          mul2(p[2], p[3], p[2], p[3], g.z, g.w);
+      for (int i = 0; i < VEC; i += Q) {
+        float* x = &v[j * VEC + i];
+        float g[Q], b[Q];
+        auto table = [&](float (&d)[Q], const float* src, float none) {
+          if constexpr (Q == 4) {
+            const float4 f = src ? __ldg(reinterpret_cast<const float4*>(src + at * VEC + i)) : make_float4(none, none, none, none);
+            d[0] = f.x, d[1] = f.y, d[2] = f.z, d[3] = f.w;
+          } else {
+#pragma unroll
+            for (int k = 0; k < Q; k++) d[k] = src ? __ldg(src + at * VEC + i + k) : none;
+          }
+        };
+        table(g, gamma, 1.0f);
+        if (beta) table(b, beta, 0.0f);
+#pragma unroll
+        for (int k = 0; k < Q; k += S) {
+          mul_s<S>(x + k, inv, inv);
+          if (beta)
+            fma_s<S>(x + k, x + k, g[k], g[k + S - 1], &b[k]);
+          else
+            mul_s<S>(x + k, g[k], g[k + S - 1]);
         }
       }
     }
@@ -113,13 +162,17 @@ __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const f
 // A row's inputs are asked for one row ahead: the next y (or the first kAhead choices' rows, whose slots
 // are asked for two rows ahead) while this row is normed, the next residual once this one is used.
 constexpr int kAhead = 2;
-// Blocks an SM, by the registers that a row's vectors need (two choices' rows and a residual in flight).
-// 16384 x 8 x 768 combine: 55 us with 2, 50 with 3; 65536 x 768 norms: 78 with 2, 90 with 3, which spills.
-template <int NV, bool COMBINE>
-constexpr int kMinBlocks = NV == 1 ? 4 : NV == 2 || (COMBINE && NV == 3) ? 3 : 2;
-template <typename T, int NV, int WPR, bool COMBINE>
-__global__ void __launch_bounds__(kThreads, kMinBlocks<NV, COMBINE>) k_block_norm(const NormArgs a) {
-  constexpr int VEC = 16 / sizeof(T), TPR = 32 * WPR, TEAMS = kThreads / TPR;
+// Blocks an SM, by the registers that a row's vectors need (two choices' rows and a residual in flight):
+// 65536 x 768 norms take 78 us with 2, 90 with 3, which spills.
+template <int VEC, int NV>
+constexpr int kMinBlocks = VEC <= 2 || NV > 2 ? 2 : NV == 2 ? 3 : 4;
+template <typename T, int VEC, int NV, int WPR, bool COMBINE>
+__global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(const NormArgs a) {
+  constexpr int TPR = 32 * WPR, TEAMS = kThreads / TPR;
+  constexpr int S = VEC == 1 ? 1 : 2;
+  typedef Pack<T, VEC> P;
+  typedef decltype(P::q) Raw;
+  static_assert(NV * VEC % 2 == 0, "sums go in pairs");
   constexpr int NY = COMBINE ? kAhead : 1;
   __shared__ float red[kTurns][8];
   int turn = 0;
@@ -127,9 +180,9 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<NV, COMBINE>) k_block_nor
   const int nvec = a.cols / VEC;
   const int64_t step = (int64_t)gridDim.x * TEAMS;
   int64_t row = (int64_t)blockIdx.x * TEAMS + team;
-  Pack<T> py[NY][NV], pr[NV];
-  auto load = [&](Pack<T> (&p)[NV], const void* base, int64_t r) {
-    const uint4* src = reinterpret_cast<const uint4*>(base) + r * nvec + t;
+  P py[NY][NV], pr[NV];
+  auto load = [&](P (&p)[NV], const void* base, int64_t r) {
+    const Raw* src = reinterpret_cast<const Raw*>(base) + r * nvec + t;
 #pragma unroll
     for (int j = 0; j < NV; j++)
       if (j * TPR + t < nvec) p[j].q = src[j * TPR];
@@ -164,20 +217,20 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<NV, COMBINE>) k_block_nor
   if (a.residual && row < a.rows) load(pr, a.residual, row);
   for (; row < a.rows; row += step) {
     float v[NV * VEC];
-    auto add = [&](const Pack<T> (&p)[NV], float scale) {
+    auto add = [&](const P (&p)[NV], float scale) {
 #pragma unroll
       for (int j = 0; j < NV; j++)
         if (j * TPR + t < nvec) {
 #pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            float* o = &v[j * VEC + i];
-            fma2(o[0], o[1], to_f<T>(p[j].t[i]), to_f<T>(p[j].t[i + 1]), scale, scale, o[0], o[1]);
+          for (int i = 0; i < VEC; i += S) {
+            const float f[2] = {to_f<T>(p[j].t[i]), to_f<T>(p[j].t[i + S - 1])};
+            fma_s<S>(&v[j * VEC + i], f, scale, scale, &v[j * VEC + i]);
           }
         }
     };
-    Pack<T> pg[NV];
+    P pg[NV];
     if (a.gate) {
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_step) + t;
+      const Raw* src = reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_step) + t;
 #pragma unroll
       for (int j = 0; j < NV; j++)
         if (j * TPR + t < nvec) pg[j].q = src[j * TPR];
@@ -211,10 +264,7 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<NV, COMBINE>) k_block_nor
       for (int j = 0; j < NV; j++)
         if (j * TPR + t < nvec) {
 #pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            float* o = &v[j * VEC + i];
-            mul2(o[0], o[1], o[0], o[1], to_f<T>(pg[j].t[i]), to_f<T>(pg[j].t[i + 1]));
-          }
+          for (int i = 0; i < VEC; i += S) mul_s<S>(&v[j * VEC + i], to_f<T>(pg[j].t[i]), to_f<T>(pg[j].t[i + S - 1]));
         }
     }
     if (a.branch_scale != 1.0f) {
@@ -226,11 +276,11 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<NV, COMBINE>) k_block_nor
       if (row + step < a.rows) load(pr, a.residual, row + step);
     }
     auto store = [&](void* to) {
-      uint4* dst = reinterpret_cast<uint4*>(to) + row * nvec + t;
+      Raw* dst = reinterpret_cast<Raw*>(to) + row * nvec + t;
 #pragma unroll
       for (int j = 0; j < NV; j++) {
         if (j * TPR + t < nvec) {
-          Pack<T> o;
+          P o;
 #pragma unroll
           for (int i = 0; i < VEC; i++) o.t[i] = from_f<T>(v[j * VEC + i]);
           dst[j * TPR] = o.q;
@@ -313,38 +363,53 @@ __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs 
   }
 }
 
-template <typename T, int NV, int WPR, bool COMBINE>
+template <typename T, int VEC, int NV, int WPR, bool COMBINE>
 int32_t launch_vec(Ctx* c, const NormArgs& a) {
   constexpr int TEAMS = kThreads / (32 * WPR);
   // As few teams as walk the rows in the same number of turns.
-  const int64_t most = (int64_t)c->num_sms * kMinBlocks<NV, COMBINE> * TEAMS;
+  const int64_t most = (int64_t)c->num_sms * kMinBlocks<VEC, NV> * TEAMS;
   const int64_t turns = (a.rows + most - 1) / most;
   const int64_t blocks = (a.rows + turns * TEAMS - 1) / (turns * TEAMS);
-  FL_CUDA(c, launch_pdl(k_block_norm<T, NV, WPR, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
+  FL_CUDA(c, launch_pdl(k_block_norm<T, VEC, NV, WPR, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
 }
 
+// Widths that 16 bytes do not divide: pairs or single elements, more of them a lane.
+template <typename T, int VEC, bool COMBINE>
+int32_t launch_narrow(Ctx* c, const NormArgs& a) {
+  const int nvec = a.cols / VEC;
+  if (nvec <= 256) return launch_vec<T, VEC, 8, 1, COMBINE>(c, a);
+  if (nvec <= 1024) return launch_vec<T, VEC, 16, 2, COMBINE>(c, a);
+  return launch_vec<T, VEC, 16, 8, COMBINE>(c, a);
+}
+constexpr int kNarrowMost = 16 * 256;
+
 template <typename T, bool COMBINE>
 int32_t launch_norm(Ctx* c, const NormArgs& a) {
   constexpr int VEC = 16 / sizeof(T);
-  const void* ptrs[] = {a.y, a.residual, a.gate, a.u, a.h, a.post_gamma, a.post_beta, a.pre_gamma, a.pre_beta};
-  bool vec = a.cols % VEC == 0;
-  for (const void* p : ptrs) vec = vec && ((uintptr_t)p & 15) == 0;
+  uintptr_t tensors = 0, tables = 0;
+  for (const void* p : {a.y, a.residual, a.gate, (const void*)a.u, (const void*)a.h}) tensors |= (uintptr_t)p;
+  for (const float* p : {a.post_gamma, a.post_beta, a.pre_gamma, a.pre_beta}) tables |= (uintptr_t)p;
   const int nvec = a.cols / VEC;
-  if (vec && nvec <= 1024) {
-    // The fewest warps a row whose lanes hold at most four vectors each.
-    if (nvec <= 32) return launch_vec<T, 1, 1, COMBINE>(c, a);
-    if (nvec <= 64) return launch_vec<T, 2, 1, COMBINE>(c, a);
-    if (nvec <= 96) return launch_vec<T, 3, 1, COMBINE>(c, a);
-    if (nvec <= 128) return launch_vec<T, 4, 1, COMBINE>(c, a);
-    if (nvec <= 192) return launch_vec<T, 3, 2, COMBINE>(c, a);
-    if (nvec <= 256) return launch_vec<T, 4, 2, COMBINE>(c, a);
-    if (nvec <= 384) return launch_vec<T, 3, 4, COMBINE>(c, a);
-    if (nvec <= 512) return launch_vec<T, 4, 4, COMBINE>(c, a);
-    if (nvec <= 768) return launch_vec<T, 3, 8, COMBINE>(c, a);
-    return launch_vec<T, 4, 8, COMBINE>(c, a);
+  if (a.cols % VEC == 0 && ((tensors | tables) & 15) == 0 && nvec <= 1024) {
+    // The fewest warps a row whose lanes hold at most four vectors each (two vectors in twice the warps:
+    // 49152 x 1024 in 87 us against 79, 65536 x 768 in 102 against 80).
+    if (nvec <= 32) return launch_vec<T, VEC, 1, 1, COMBINE>(c, a);
+    if (nvec <= 64) return launch_vec<T, VEC, 2, 1, COMBINE>(c, a);
+    if (nvec <= 96) return launch_vec<T, VEC, 3, 1, COMBINE>(c, a);
+    if (nvec <= 128) return launch_vec<T, VEC, 4, 1, COMBINE>(c, a);
+    if (nvec <= 192) return launch_vec<T, VEC, 3, 2, COMBINE>(c, a);
+    if (nvec <= 256) return launch_vec<T, VEC, 4, 2, COMBINE>(c, a);
+    if (nvec <= 384) return launch_vec<T, VEC, 3, 4, COMBINE>(c, a);
+    if (nvec <= 512) return launch_vec<T, VEC, 4, 4, COMBINE>(c, a);
+    if (nvec <= 768) return launch_vec<T, VEC, 3, 8, COMBINE>(c, a);
+    return launch_vec<T, VEC, 4, 8, COMBINE>(c, a);
   }
+  if constexpr (sizeof(T) == 2) {
+    if (a.cols % 2 == 0 && (tensors & 3) == 0 && a.cols <= 2 * kNarrowMost) return launch_narrow<T, 2, COMBINE>(c, a);
+  }
+  if (a.cols <= kNarrowMost) return launch_narrow<T, 1, COMBINE>(c, a);
   auto kern = k_block_norm_generic<T, COMBINE>;
   const int smem = a.cols * 4;
   static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
