@@ -185,7 +185,16 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
     const Raw* src = reinterpret_cast<const Raw*>(base) + r * nvec + t;
 #pragma unroll
     for (int j = 0; j < NV; j++)
-      if (j * TPR + t < nvec) p[j].q = src[j * TPR];
+      if (j * TPR + t < nvec) {
+        // A one-warp row's choices pass by L1, which keeps gamma and beta (32768 x 2 x 768: 39 us against
+        // 43; rows of several warps are slower with it, 32768 x 1 x 2048 102 against 94).
+        if constexpr (COMBINE && WPR == 1 && VEC * sizeof(T) == 16)
+          asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(p[j].q.x), "=r"(p[j].q.y), "=r"(p[j].q.z), "=r"(p[j].q.w)
+                       : "l"(src + j * TPR));
+        else
+          p[j].q = src[j * TPR];
+      }
   };
   // Combine: lane j < top_k holds choice j of the current and of the next row.
   int32_t slot = -1, slot_next = -1;

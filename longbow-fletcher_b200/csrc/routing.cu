@@ -13,9 +13,9 @@
 // Grouping is a stable counting sort in two launches: k_route leaves, per block of rows, how many
 // choices each expert got, and its last block to finish turns these into what precedes each block;
 // k_group ranks its pairs within the block and writes slots and their inverse.  (Summed by every
-// block of k_group instead, the same lines of L2 are read by all at once: 9 of 19 us.)  Up to
-// kOneBlockPairs pairs one block does all in one launch.  Which block is last changes nothing in the
-// result, so the slots are the same in every run.
+// block of k_group instead, the same lines of L2 are read by all at once: 9 of 19 us.)  Where a cluster
+// of blocks can hold all pairs, its blocks read one another's counts and one launch does it all.
+// Nothing in the result depends on which block is last, so the slots are the same in every run.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -344,10 +344,21 @@ __device__ __forceinline__ int32_t scan_experts(const int32_t* n, int32_t* at, i
   return total;
 }
 
-// ONE: a single block, which groups its (at most kSub) pairs too.
+__device__ __forceinline__ int32_t load_shared_of(const int32_t* p, uint32_t rank) {
+  int32_t v;
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.s32 %0, [a];\n}"
+               : "=r"(v)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank)
+               : "memory");
+  return v;
+}
+
+// ONE: a cluster of up to kClusterMost blocks, with at most kSub pairs each, which see one another's counts
+// and so group their pairs too.
+constexpr int kClusterMost = 8;
 template <typename T, int L, int KM, bool ONE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArgs a) {
-  __shared__ int32_t hist[kMaxExperts];
+  __shared__ int32_t hist[kMaxExperts], at[kMaxExperts], tmp[kWarps + 1];
   extern __shared__ int32_t dyn[];  // ONE: count [kWarps][E], ids [kSub]
   int16_t* ids = ONE ? reinterpret_cast<int16_t*>(dyn + kWarps * a.E) : nullptr;
   for (int e = threadIdx.x; e < a.E; e += kThreads) hist[e] = 0;
@@ -360,19 +371,42 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
     } else {
       for (int64_t p = r0 * a.k + threadIdx.x; p < r1 * a.k; p += kThreads) {
         const int e = a.experts[p];
-        if (ONE) ids[p] = (int16_t)e;
+        if (ONE) ids[p - r0 * a.k] = (int16_t)e;
         if (e >= 0) atomicAdd(&hist[e], 1);
       }
     }
   }
-  __syncthreads();
   if constexpr (ONE) {
-    __shared__ int32_t at[kMaxExperts], tmp[kWarps + 1];
-    const int32_t total = scan_experts(hist, at, a.E, tmp);
-    for (int e = threadIdx.x; e < a.E; e += kThreads) a.offsets[e] = at[e];
-    if (threadIdx.x == 0) a.offsets[a.E] = total;
-    assign_slots(a, 0, (int)(r1 * a.k), ids, at, dyn);
+    __shared__ int32_t all[kMaxExperts], before[kMaxExperts];
+    const bool cluster = gridDim.x > 1;  // the grid is the cluster
+    if (cluster)
+      asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else
+      __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += kThreads) {
+      int32_t n = 0, b = 0;
+      for (uint32_t r = 0; r < gridDim.x; r++) {
+        const int32_t v = cluster ? load_shared_of(&hist[e], r) : hist[e];
+        n += v;
+        if (r < blockIdx.x) b += v;
+      }
+      all[e] = n;
+      before[e] = b;
+    }
+    if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' counts are read
+    __syncthreads();
+    const int32_t total = scan_experts(all, at, a.E, tmp);
+    if (blockIdx.x == 0) {
+      for (int e = threadIdx.x; e < a.E; e += kThreads) a.offsets[e] = at[e];
+      if (threadIdx.x == 0) a.offsets[a.E] = total;
+      __syncthreads();
+    }
+    for (int e = threadIdx.x; e < a.E; e += kThreads) at[e] += before[e];
+    __syncthreads();
+    if (r0 < r1) assign_slots(a, r0 * a.k, (int)((r1 - r0) * a.k), ids, at, dyn);
+    if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody reads this block's now
   } else {
+    __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += kThreads) a.hist[(int64_t)e * a.stride + blockIdx.x] = hist[e];
     __shared__ bool last;
     __threadfence();
@@ -381,31 +415,49 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
     __syncthreads();
     if (!last) return;
     __threadfence();
-    __shared__ int32_t at[kMaxExperts], tmp[kWarps + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
     if (threadIdx.x == 0) *a.ticket = 0;
-    // A warp an expert: counts become exclusive sums over the blocks, four a lane.
-    for (int e = warp; e < a.E; e += kWarps) {
-      int4* row = reinterpret_cast<int4*>(a.hist + (int64_t)e * a.stride);
-      int32_t carry = 0;
-#pragma unroll 4
-      for (int i = lane; i - lane < (blocks + 3) / 4; i += 32) {
-        int4 v = 4 * i < blocks ? __ldcg(row + i) : make_int4(0, 0, 0, 0);
-        if (4 * i + 1 >= blocks) v.y = 0;
-        if (4 * i + 2 >= blocks) v.z = 0;
-        if (4 * i + 3 >= blocks) v.w = 0;
-        const int32_t n = v.x + v.y + v.z + v.w;
-        int32_t s = n;
+    // Counts become exclusive sums over the blocks: a warp an expert, four blocks a lane, the counts of
+    // four experts on their way at once.
+    constexpr int TURNS = 3, AT_ONCE = 4;  // 3 * 128 >= max_blocks
+    const int quads = (blocks + 3) / 4;
+    for (int e0 = warp; e0 < a.E; e0 += AT_ONCE * kWarps) {
+      int4 v[AT_ONCE][TURNS];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
-          if (lane >= o) s += u;
+      for (int q = 0; q < AT_ONCE; q++)
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) {
+          const int e = e0 + q * kWarps, at4 = i * 32 + lane;
+          v[q][i] = e < a.E && at4 < quads ? __ldcg(reinterpret_cast<const int4*>(a.hist + (int64_t)e * a.stride) + at4)
+                                           : make_int4(0, 0, 0, 0);
         }
-        const int32_t b = carry + s - n;
-        if (4 * i < blocks) row[i] = make_int4(b, b + v.x, b + v.x + v.y, b + v.x + v.y + v.z);
-        carry += __shfl_sync(0xffffffffu, s, 31);
+#pragma unroll
+      for (int q = 0; q < AT_ONCE; q++) {
+        const int e = e0 + q * kWarps;
+        if (e >= a.E) break;
+        int32_t carry = 0;
+#pragma unroll
+        for (int i = 0; i < TURNS; i++) {
+          const int at4 = i * 32 + lane;
+          int4 n = v[q][i];
+          if (4 * at4 + 1 >= blocks) n.y = 0;  // behind the last block
+          if (4 * at4 + 2 >= blocks) n.z = 0;
+          if (4 * at4 + 3 >= blocks) n.w = 0;
+          const int32_t mine = n.x + n.y + n.z + n.w;
+          int32_t s = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+          }
+          const int32_t b = carry + s - mine;
+          if (at4 < quads)
+            reinterpret_cast<int4*>(a.hist + (int64_t)e * a.stride)[at4] =
+                make_int4(b, b + n.x, b + n.x + n.y, b + n.x + n.y + n.z);
+          carry += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) hist[e] = carry;
       }
-      if (lane == 0) hist[e] = carry;
     }
     __syncthreads();
     const int32_t total = scan_experts(hist, at, a.E, tmp);
@@ -434,14 +486,25 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArg
   }
 }
 
-constexpr int64_t kOneBlockPairs = 2048;
-static_assert(kOneBlockPairs <= kSub, "one block's pairs");
-
 template <typename T, int L, int KM>
-int32_t route_l(Ctx* c, const RouteArgs& a, int blocks) {
+int32_t route_l(Ctx* c, const RouteArgs& a, int blocks, bool one) {
   const size_t smem = (size_t)kWarps * a.E * 4;  // at most 16 KB
-  if (blocks == 1) {
-    FL_CUDA(c, launch_pdl(k_route<T, L, KM, true>, dim3(1), dim3(kThreads), smem + kSub * 2, c->stream, a));
+  if (one) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = blocks;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem + kSub * 2;
+    cfg.stream = c->stream;
+    cfg.attrs = at;
+    cfg.numAttrs = blocks > 1 ? 2 : 1;
+    FL_CUDA(c, cudaLaunchKernelEx(&cfg, k_route<T, L, KM, true>, a));
     FL_LAUNCH(c);
     return FLETCHER_OK;
   }
@@ -453,22 +516,25 @@ int32_t route_l(Ctx* c, const RouteArgs& a, int blocks) {
 }
 
 template <typename T, int L>
-int32_t route_k(Ctx* c, const RouteArgs& a, int blocks) {
-  if (a.k <= 2) return route_l<T, L, 2>(c, a, blocks);
-  if (a.k <= 8) return route_l<T, L, 8>(c, a, blocks);
-  return route_l<T, L, 16>(c, a, blocks);
+int32_t route_k(Ctx* c, const RouteArgs& a, int blocks, bool one) {
+  if (a.k <= 2) return route_l<T, L, 2>(c, a, blocks, one);
+  if (a.k <= 8) return route_l<T, L, 8>(c, a, blocks, one);
+  return route_l<T, L, 16>(c, a, blocks, one);
 }
 
 // Lanes a row: one where a chunk holds all experts; a warp for few rows of many.
 int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E <= 4 * V || a.rows > 2 * kThreads / 32 ? 4 : 32; }
 
 template <typename T>
-int32_t route_t(Ctx* c, const RouteArgs& a, int blocks) {
+int32_t route_t(Ctx* c, const RouteArgs& a, int blocks, bool one) {
   const int lanes = lanes_of(a);
-  return lanes == 1 ? route_k<T, 1>(c, a, blocks) : lanes == 4 ? route_k<T, 4>(c, a, blocks) : route_k<T, 32>(c, a, blocks);
+  return lanes == 1   ? route_k<T, 1>(c, a, blocks, one)
+         : lanes == 4 ? route_k<T, 4>(c, a, blocks, one)
+                      : route_k<T, 32>(c, a, blocks, one);
 }
 
-int max_blocks(const Ctx* c) { return kBlocksPerSM * c->num_sms / 4 * 4; }  // rows of int4
+// Rows of int4, at most what the last block's lanes hold.
+int max_blocks(const Ctx* c) { return std::min(kBlocksPerSM * c->num_sms / 4 * 4, 3 * 128); }
 
 int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   Ctx* c = r->c;
@@ -482,19 +548,24 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   a.hist = r->hist;
   a.ticket = r->ticket;
   a.stride = max_blocks(c);
-  const int64_t pairs = a.rows * a.k;
-  // A block for every 256 pairs, to keep short batches wide, up to two blocks an SM.
-  const int64_t want = pairs <= kOneBlockPairs ? 1 : (pairs + 255) / 256;
-  int blocks = (int)std::min<int64_t>(want, max_blocks(c));
-  a.chunk = (a.rows + blocks - 1) / blocks;
-  if (blocks > 1) {  // whole passes of a block's threads
-    const int64_t pass = kThreads / lanes_of(a);
-    a.chunk = (a.chunk + pass - 1) / pass * pass;
-    blocks = (int)((a.rows + a.chunk - 1) / a.chunk);
+  const int64_t pass = kThreads / lanes_of(a);  // rows a block takes at once
+  const int64_t passes = std::max<int64_t>(1, (a.rows + pass - 1) / pass);
+  // One launch where a cluster's blocks hold the pairs and take no more than two turns (4096 x 64 -> 6 in
+  // four turns: 16.8 us, in two launches 10.7; 4096 x 8 -> 2: 5.7 against 9.0).
+  const int64_t fit = (a.rows + kSub / a.k - 1) / (kSub / a.k);  // blocks of at most kSub pairs
+  const bool one = fit <= kClusterMost && passes <= 2 * kClusterMost;
+  int64_t blocks = std::max(fit, std::min<int64_t>(passes, one ? kClusterMost : max_blocks(c)));
+  if (one) {
+    a.chunk = (a.rows + blocks - 1) / blocks;
+  } else {
+    blocks = std::min<int64_t>(blocks, max_blocks(c));
+    a.chunk = ((a.rows + blocks - 1) / blocks + pass - 1) / pass * pass;  // whole turns
+    blocks = (a.rows + a.chunk - 1) / a.chunk;
   }
-  if (dtype == FLETCHER_BF16) return route_t<__nv_bfloat16>(c, a, blocks);
-  if (dtype == FLETCHER_F16) return route_t<__half>(c, a, blocks);
-  return route_t<float>(c, a, blocks);
+  const int n = (int)blocks;
+  if (dtype == FLETCHER_BF16) return route_t<__nv_bfloat16>(c, a, n, one);
+  if (dtype == FLETCHER_F16) return route_t<__half>(c, a, n, one);
+  return route_t<float>(c, a, n, one);
 }
 
 }  // namespace
