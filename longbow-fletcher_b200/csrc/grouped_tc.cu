@@ -441,7 +441,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Few rows a group: the weights' bytes are the work, so a tile takes at most 32 rows of x (4 KB a slab next
 // to 16 KB of W; the MMA's other 96 rows read whatever lies behind and are never looked at), rows of
 // tokens are gathered by TMA in quads, only as many as there are, and the rest of shared memory is a
-// deep ring of W.  Warps 0 and 4 drain lanes 0-31 of the accumulator, half the columns each.
+// deep ring of W.  Warps 0 and 4 drain lanes 0-31 of the accumulator, half the columns each.  Where the
+// tiles are too few for the SMs (a row or two), the slabs of a tile are split between the CTAs of a
+// cluster (SPLIT), which add their sums through distributed shared memory.
 struct SmallCfg {
   static constexpr int TILE_M = 32, BN = 128;
   static constexpr int kThreads = 160;
@@ -458,6 +460,12 @@ struct SmallCfg {
   static_assert(STAGES * B_BYTES >= BM * BK * 2, "the MMA reads 128 rows from the last slab of x on");
 };
 
+__device__ __forceinline__ uint32_t cluster_ctas() {
+  uint32_t n;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+
 // Four rows of a 2-D tensor by index, 64 columns from x, one below the other.
 __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, uint64_t* bar, int x, const int (&r)[4]) {
   asm volatile(
@@ -467,7 +475,7 @@ __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-template <typename T, bool GATED, bool GATHER>
+template <typename T, bool GATED, bool GATHER, bool SPLIT>
 __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
     k_grouped_small(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
   using C = SmallCfg;
@@ -511,6 +519,11 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
   }
   pdl_wait();  // the routing and x are the previous kernels' work
   const int num_tiles = fill_table(args.offsets, args.E, C::TILE_M, offs, tmp) * args.n_tiles;
+  // SPLIT: this CTA's tile (its cluster's) and range of K slabs; else all tiles with a stride, all slabs.
+  const int ranks = SPLIT ? (int)cluster_ctas() : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
+  const int first_tile = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
+  const int tile_stride = SPLIT ? num_tiles : (int)gridDim.x;
+  const int kb0 = SPLIT ? args.num_kb * rank / ranks : 0, kb1 = SPLIT ? args.num_kb * (rank + 1) / ranks : args.num_kb;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -521,7 +534,7 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
     int stage = 0;
     uint32_t phase = 0, issued = 0, issued_par = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
       const Tile t = walk.at(tile);
       const int quads = GATHER ? (min(t.end - t.first, C::TILE_M) + 3) / 4 : 0;
       int rows[4] = {};
@@ -532,7 +545,7 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
           rows[i] = args.pair_of[s < t.end ? s : t.first] / args.top_k;  // past the group: computed, not stored
         }
       }
-      for (int kb = 0; kb < args.num_kb; kb++) {
+      for (int kb = kb0; kb < kb1; kb++) {
         ok = __all_sync(0xffffffffu, mbar_wait_spin(&empty[stage], phase ^ 1, abort, args.err));
         if (!ok) break;
         uint8_t* a = sA + stage * C::A_BYTES;
@@ -564,19 +577,19 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride, ++it) {
         const int acc = it & 1;
         if (!mbar_wait_spin(&tempty[acc], ((it >> 1) & 1) ^ 1, abort, args.err)) break;
         tc_fence_after();
         const uint32_t d = tmem_base + acc * BN;
-        for (int kb = 0; kb < args.num_kb; kb++) {
+        for (int kb = kb0; kb < kb1; kb++) {
           if (!(ok = mbar_wait_spin(&full[stage], phase, abort, args.err))) break;
           tc_fence_after();
           const uint64_t da = sw128_desc(smem_u32(sA + stage * C::A_BYTES));
           const uint64_t db = desc_mn(smem_u32(sB + stage * C::B_BYTES));
 #pragma unroll
           for (int k = 0; k < BK / 16; k++)
-            mma_f16(d, da + 2 * k, db + (uint64_t)k * (2048 >> 4), id, (kb | k) != 0);
+            mma_f16(d, da + 2 * k, db + (uint64_t)k * (2048 >> 4), id, kb > kb0 || k > 0);
           mma_commit(&empty[stage]);
           if (++stage == C::STAGES) {
             stage = 0;
@@ -591,20 +604,44 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
         mbar_drain(drain, 0);
       }
     }
-  } else if (warp == 0 || warp == 4) {
-    const int half = warp >> 2;
-    constexpr int COLS = OUT_N / 2;  // this warp's output columns: 32 (gated) or 64
-    T* out = reinterpret_cast<T*>(args.out);
+  }
+  // Warps 0 and 4: bias, activation and rows of a tile's half, from v (gated: 32 gates, 32 ups).
+  constexpr int COLS = OUT_N / 2;  // this warp's output columns: 32 (gated) or 64
+  const int half = warp >> 2, c0 = half * COLS;
+  auto finish = [&](const Tile& t, float (&v)[64]) {
+    float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
+    float (&hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
+    const int64_t ocol = (int64_t)t.nb * OUT_N + c0;
+    if (args.bias) {
+      const T* bias = reinterpret_cast<const T*>(args.bias) + (int64_t)t.e * args.N;
+      add_bias32<T>(lo, bias, ocol, args.n_out);
+      if constexpr (GATED)
+        add_bias32<T>(hi, bias + args.n_out, ocol, args.n_out);
+      else
+        add_bias32<T>(hi, bias, ocol + 32, args.n_out);
+    }
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < 32; i++) v[i] = silu16(v[i]) * v[32 + i];
+    } else if (args.act == FLETCHER_ACT_GELU) {
+#pragma unroll
+      for (int i = 0; i < 64; i += 2) gelu_pair(v[i], v[i + 1]);
+    }
+    if (t.first + lane < t.end) {
+      T* dst = reinterpret_cast<T*>(args.out) + (int64_t)(t.first + lane) * args.n_out + ocol;
+#pragma unroll
+      for (int j = 0; j < COLS / 8; j++)
+        if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
+    }
+  };
+  if (!SPLIT && (warp == 0 || warp == 4)) {
     int it = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
+    for (int tile = first_tile; tile < num_tiles; tile += tile_stride, ++it) {
       const Tile t = walk.at(tile);
       const int acc = it & 1;
       const uint32_t tbase = tmem_base + acc * BN;
-      const T* bias = args.bias ? reinterpret_cast<const T*>(args.bias) + (int64_t)t.e * args.N : nullptr;
       if (!mbar_wait_spin(&tfull[acc], (it >> 1) & 1, abort, args.err)) break;
       tc_fence_after();
-      const int c0 = half * COLS;
-      const int64_t ocol = (int64_t)t.nb * OUT_N + c0;
       float v[64];
       float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
       float (&hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
@@ -612,27 +649,52 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty[acc]);
-      if (bias) {
-        add_bias32<T>(lo, bias, ocol, args.n_out);
-        if constexpr (GATED)
-          add_bias32<T>(hi, bias + args.n_out, ocol, args.n_out);
-        else
-          add_bias32<T>(hi, bias, ocol + 32, args.n_out);
-      }
-      if constexpr (GATED) {
+      finish(t, v);
+    }
+  }
+  if constexpr (SPLIT) {
+    // The other ranks leave their sums in shared memory, over the ring, which is done with; rank 0 adds them in
+    // their order.  Every thread takes both cluster barriers, whatever happened before them.
+    constexpr int PITCH = 64 + 4;  // floats of a row of a warp's half
+    float* mine = reinterpret_cast<float*>(smem) + (half * C::TILE_M + lane) * PITCH;
+    float v[64];
+    Tile t{};
+    bool have = false;
+    __syncwarp();
+    if ((warp == 0 || warp == 4) && first_tile < num_tiles) {
+      t = walk.at(first_tile);
+      have = mbar_wait_spin(&tfull[0], 0, abort, args.err);
+      have = __all_sync(0xffffffffu, have);
+      if (have) {
+        tc_fence_after();
+        float (&lo)[32] = *reinterpret_cast<float(*)[32]>(&v[0]);
+        float (&hi)[32] = *reinterpret_cast<float(*)[32]>(&v[32]);
+        tmem_ld32x2(tmem_base + c0, tmem_base + c0 + (GATED ? OUT_N : 32), lo, hi);
+        if (rank > 0 && t.first + lane < t.end) {
 #pragma unroll
-        for (int i = 0; i < 32; i++) v[i] = silu16(v[i]) * v[32 + i];
-      } else if (args.act == FLETCHER_ACT_GELU) {
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) gelu_pair(v[i], v[i + 1]);
-      }
-      if (t.first + lane < t.end) {
-        T* dst = out + (int64_t)(t.first + lane) * args.n_out + ocol;
-#pragma unroll
-        for (int j = 0; j < COLS / 8; j++)
-          if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
+          for (int i = 0; i < 64; i += 4) *reinterpret_cast<float4*>(mine + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
       }
     }
+    cluster_sync();
+    if (rank == 0 && have) {
+      if (t.first + lane < t.end) {
+        for (int r = 1; r < ranks; r++) {
+          const uint32_t src = mapa_shared(smem_u32(mine), r);
+#pragma unroll
+          for (int i = 0; i < 64; i += 4) {
+            float4 q;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(q.x), "=f"(q.y), "=f"(q.z), "=f"(q.w)
+                         : "r"(src + i * 4)
+                         : "memory");
+            v[i] += q.x, v[i + 1] += q.y, v[i + 2] += q.z, v[i + 3] += q.w;
+          }
+        }
+      }
+      finish(t, v);
+    }
+    cluster_sync();  // rank 0 has read the others' sums
   }
 
   tc_fence_before();
@@ -665,8 +727,8 @@ int64_t most_tiles(const GroupedArgs& g, int tile_m, int n_tiles) {
   return (g.pairs / tile_m + std::min<int64_t>(g.experts, g.pairs)) * n_tiles;
 }
 
-template <typename T, bool GATED, bool GATHER>
-int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g) {
+template <typename T, bool GATED, bool GATHER, bool SPLIT>
+int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g, int ranks) {
   using C = SmallCfg;
   CUtensorMap ma, mb;
   int32_t rc;
@@ -675,24 +737,48 @@ int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g) {
     return rc;
   if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
   const Args a = args_of(c, g, GATED ? C::BN / 2 : C::BN);
-  auto kern = k_grouped_small<T, GATED, GATHER>;
+  auto kern = k_grouped_small<T, GATED, GATHER, SPLIT>;
   static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
   if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
     FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_set[c->device & 63].store(true, std::memory_order_release);
   }
-  const int64_t grid = std::min<int64_t>(most_tiles(g, C::TILE_M, a.n_tiles), c->num_sms);
-  FL_CUDA(c, launch_pdl(kern, dim3((unsigned)grid), dim3(C::kThreads), C::SMEM, c->stream, ma, mb, a));
+  const int64_t tiles = most_tiles(g, C::TILE_M, a.n_tiles);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = ranks;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(SPLIT ? tiles * ranks : std::min<int64_t>(tiles, c->num_sms)));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = c->stream;
+  cfg.attrs = at;
+  cfg.numAttrs = SPLIT ? 2 : 1;
+  FL_CUDA(c, cudaLaunchKernelEx(&cfg, kern, ma, mb, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
+}
+
+template <typename T, bool GATED, bool GATHER>
+int32_t launch_small_g(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  // CTAs a tile: as many as the SMs have room for, at most 8, two slabs of K each at least.
+  const int out_n = GATED ? SmallCfg::BN / 2 : SmallCfg::BN;
+  const int64_t tiles = most_tiles(g, SmallCfg::TILE_M, (int)((g.n_out + out_n - 1) / out_n));
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks * 2 <= c->num_sms && g.K >= ranks * 4 * BK) ranks *= 2;
+  return ranks > 1 ? run_small<T, GATED, GATHER, true>(c, dt, g, ranks) : run_small<T, GATED, GATHER, false>(c, dt, g, 1);
 }
 
 template <typename T>
 int32_t launch_small(Ctx* c, int32_t dt, const GroupedArgs& g) {
   const bool gather = g.pair_of != nullptr;
   if (g.act == FLETCHER_ACT_SWIGLU)
-    return gather ? run_small<T, true, true>(c, dt, g) : run_small<T, true, false>(c, dt, g);
-  return gather ? run_small<T, false, true>(c, dt, g) : run_small<T, false, false>(c, dt, g);
+    return gather ? launch_small_g<T, true, true>(c, dt, g) : launch_small_g<T, true, false>(c, dt, g);
+  return gather ? launch_small_g<T, false, true>(c, dt, g) : launch_small_g<T, false, false>(c, dt, g);
 }
 
 template <typename T, int BN, bool PAIR, bool GATED>

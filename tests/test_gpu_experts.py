@@ -243,7 +243,8 @@ def run_grouped(fl, be, rows, experts, k, K, N, act, dtype, bias, grouped_input,
 
 SHAPES = [  # rows, experts, k, K, N
     (1, 8, 2, 64, 128), (1, 1, 1, 8, 16), (3, 4, 1, 72, 40), (16, 64, 4, 256, 192), (33, 5, 2, 200, 264),
-    (130, 3, 2, 136, 512), (257, 2, 1, 64, 256), (500, 12, 3, 320, 384), (1031, 4, 2, 128, 1032)]
+    (130, 3, 2, 136, 512), (257, 2, 1, 64, 256), (500, 12, 3, 320, 384), (1031, 4, 2, 128, 1032),
+    (1, 8, 2, 768, 1536), (2, 4, 1, 2048, 136), (20, 2, 1, 1000, 72), (40, 2, 2, 520, 64)]
 
 
 @pytest.mark.parametrize("rows,experts,k,K,N", SHAPES)
