@@ -12,6 +12,7 @@
 #include <cmath>
 
 #include "routing.cuh"
+#include "tc_common.cuh"
 
 namespace fl {
 namespace {
@@ -98,65 +99,81 @@ __device__ __forceinline__ float team_sum(float s, float (*red)[8], int& turn) {
   return s;
 }
 
+// Whether all lanes hold a vector j: in a FULL row each does, and with 4 or 8 values a vector all but the
+// last (the launch takes no more of them than the row needs).
+template <int VEC, int NV, bool FULL>
+__device__ __forceinline__ constexpr bool kWhole(int j) {
+  return FULL || (VEC >= 4 && j < NV - 1);
+}
+
 // v = norm(v) for the team's row: lane t holds vectors t, t + TPR, ...; what lies past the row is 0
-// and stays out of the sums.
-template <int VEC, int NV, int WPR>
+// and stays out of the sums.  FULL: the lanes' vectors are exactly the row.  Packed pairs of fp32, with
+// the uniform choices outside the loops: at 16-bit widths instructions weigh as much as bytes (with the
+// choices inside, 1100 instructions a row of 1024 and 78 us for 49152 rows, against 67).
+template <int VEC, int NV, int WPR, bool FULL>
 __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const float* __restrict__ gamma,
                                          const float* __restrict__ beta, float eps, int t, int nvec, int cols,
                                          float (*red)[8], int& turn) {
   constexpr int TPR = 32 * WPR;
-  if (kind == FLETCHER_NORM_NONE) return;
-  // In packed pairs of fp32: half the instructions, which at 16-bit widths weigh as much as the bytes.
   constexpr int S = VEC == 1 ? 1 : 2, Q = VEC < 4 ? S : 4;  // values a step, and a load of gamma or beta
-  float mean = 0.f;
+  if (kind == FLETCHER_NORM_NONE) return;
   if (kind == FLETCHER_NORM_LAYER) {
     float p[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV * VEC; i += 2) add2(p[0], p[1], v[i], v[i + 1]);
-    mean = team_sum<WPR>(p[0] + p[1], red, turn) / (float)cols;
-  }
-  float q[2] = {0.f, 0.f};
+    const float mean = team_sum<WPR>(p[0] + p[1], red, turn) / (float)cols;
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    if (j * TPR + t < nvec) {
+    for (int j = 0; j < NV; j++)
+      if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) {
 #pragma unroll
-      for (int i = j * VEC; i < (j + 1) * VEC; i += S) {
-        if (kind == FLETCHER_NORM_LAYER) add_s<S>(&v[i], -mean);
-        fma_s<S>(q, &v[i], v[i], S == 2 ? v[i + S - 1] : 0.f, q);
+        for (int i = j * VEC; i < (j + 1) * VEC; i += S) add_s<S>(&v[i], -mean);
       }
-    }
   }
-  const float inv = 1.0f / sqrtf(team_sum<WPR>(q[0] + q[1], red, turn) / (float)cols + eps);
+  float q[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < NV; j++) {
-    const int at = j * TPR + t;
-    if (at < nvec) {
+  for (int i = 0; i < NV * VEC; i += 2) fma2(q[i & 2], q[(i & 2) + 1], v[i], v[i + 1], v[i], v[i + 1], q[i & 2], q[(i & 2) + 1]);
+  const float inv = 1.0f / sqrtf(team_sum<WPR>((q[0] + q[1]) + (q[2] + q[3]), red, turn) / (float)cols + eps);
 #pragma unroll
-      for (int i = 0; i < VEC; i += Q) {
-        float* x = &v[j * VEC + i];
-        float g[Q], b[Q];
-        auto table = [&](float (&d)[Q], const float* src, float none) {
-          if constexpr (Q == 4) {
-            const float4 f = src ? __ldg(reinterpret_cast<const float4*>(src + at * VEC + i)) : make_float4(none, none, none, none);
-            d[0] = f.x, d[1] = f.y, d[2] = f.z, d[3] = f.w;
-          } else {
+  for (int i = 0; i < NV * VEC; i += 2) mul2(v[i], v[i + 1], v[i], v[i + 1], inv, inv);
+  auto table = [&](const float* src, float (&d)[Q], int at) {
+    if constexpr (Q == 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(src + at));
+      d[0] = f.x, d[1] = f.y, d[2] = f.z, d[3] = f.w;
+    } else {
 #pragma unroll
-            for (int k = 0; k < Q; k++) d[k] = src ? __ldg(src + at * VEC + i + k) : none;
+      for (int k = 0; k < Q; k++) d[k] = __ldg(src + at + k);
+    }
+  };
+  const float one = 1.0f;
+  auto scale = [&](auto with_gamma, auto with_beta) {
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+      if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += Q) {
+          float* x = &v[j * VEC + i];
+          float g[Q], b[Q];
+          const int at = (j * TPR + t) * VEC + i;
+          if constexpr (decltype(with_gamma)::value) table(gamma, g, at);
+          if constexpr (decltype(with_beta)::value) table(beta, b, at);
+#pragma unroll
+          for (int k = 0; k < Q; k += S) {
+            if constexpr (decltype(with_gamma)::value && decltype(with_beta)::value)
+              fma_s<S>(x + k, x + k, g[k], g[k + S - 1], &b[k]);
+            else if constexpr (decltype(with_gamma)::value)
+              mul_s<S>(x + k, g[k], g[k + S - 1]);
+            else
+              fma_s<S>(x + k, x + k, one, one, &b[k]);
           }
-        };
-        table(g, gamma, 1.0f);
-        if (beta) table(b, beta, 0.0f);
-#pragma unroll
-        for (int k = 0; k < Q; k += S) {
-          mul_s<S>(x + k, inv, inv);
-          if (beta)
-            fma_s<S>(x + k, x + k, g[k], g[k + S - 1], &b[k]);
-          else
-            mul_s<S>(x + k, g[k], g[k + S - 1]);
         }
       }
-    }
-  }
+  };
+  if (gamma && beta)
+    scale(std::true_type{}, std::true_type{});
+  else if (gamma)
+    scale(std::true_type{}, std::false_type{});
+  else if (beta)
+    scale(std::false_type{}, std::true_type{});
 }
 
 // A row's inputs are asked for one row ahead: the next y (or the first kAhead choices' rows, whose slots
@@ -166,7 +183,7 @@ constexpr int kAhead = 2;
 // 65536 x 768 norms take 78 us with 2, 90 with 3, which spills.
 template <int VEC, int NV>
 constexpr int kMinBlocks = VEC <= 2 || NV > 2 ? 2 : NV == 2 ? 3 : 4;
-template <typename T, int VEC, int NV, int WPR, bool COMBINE>
+template <typename T, int VEC, int NV, int WPR, bool FULL, bool COMBINE>
 __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(const NormArgs a) {
   constexpr int TPR = 32 * WPR, TEAMS = kThreads / TPR;
   constexpr int S = VEC == 1 ? 1 : 2;
@@ -185,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
     const Raw* src = reinterpret_cast<const Raw*>(base) + r * nvec + t;
 #pragma unroll
     for (int j = 0; j < NV; j++)
-      if (j * TPR + t < nvec) {
+      if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) {
         // A one-warp row's choices pass by L1, which keeps gamma and beta (32768 x 2 x 768: 39 us against
         // 43; rows of several warps are slower with it, 32768 x 1 x 2048 102 against 94).
         if constexpr (COMBINE && WPR == 1 && VEC * sizeof(T) == 16)
@@ -229,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
     auto add = [&](const P (&p)[NV], float scale) {
 #pragma unroll
       for (int j = 0; j < NV; j++)
-        if (j * TPR + t < nvec) {
+        if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) {
 #pragma unroll
           for (int i = 0; i < VEC; i += S) {
             const float f[2] = {to_f<T>(p[j].t[i]), to_f<T>(p[j].t[i + S - 1])};
@@ -242,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
       const Raw* src = reinterpret_cast<const Raw*>(reinterpret_cast<const T*>(a.gate) + row * a.gate_step) + t;
 #pragma unroll
       for (int j = 0; j < NV; j++)
-        if (j * TPR + t < nvec) pg[j].q = src[j * TPR];
+        if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) pg[j].q = src[j * TPR];
     }
 #pragma unroll
     for (int i = 0; i < NV * VEC; i++) v[i] = 0.f;
@@ -267,11 +284,11 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
       add(py[0], 1.0f);
     }
     load_y(row + step, slot);
-    norm_row<VEC, NV, WPR>(v, a.post, a.post_gamma, a.post_beta, a.eps, t, nvec, a.cols, red, turn);
+    norm_row<VEC, NV, WPR, FULL>(v, a.post, a.post_gamma, a.post_beta, a.eps, t, nvec, a.cols, red, turn);
     if (a.gate) {
 #pragma unroll
       for (int j = 0; j < NV; j++)
-        if (j * TPR + t < nvec) {
+        if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) {
 #pragma unroll
           for (int i = 0; i < VEC; i += S) mul_s<S>(&v[j * VEC + i], to_f<T>(pg[j].t[i]), to_f<T>(pg[j].t[i + S - 1]));
         }
@@ -288,17 +305,23 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
       Raw* dst = reinterpret_cast<Raw*>(to) + row * nvec + t;
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        if (j * TPR + t < nvec) {
+        if (kWhole<VEC, NV, FULL>(j) || j * TPR + t < nvec) {
           P o;
+          if constexpr (sizeof(T) == 2 && VEC > 1) {
 #pragma unroll
-          for (int i = 0; i < VEC; i++) o.t[i] = from_f<T>(v[j * VEC + i]);
+            for (int i = 0; i < VEC; i += 2)
+              reinterpret_cast<uint32_t*>(&o)[i / 2] = tc::pack2<T>(v[j * VEC + i], v[j * VEC + i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o.t[i] = from_f<T>(v[j * VEC + i]);
+          }
           dst[j * TPR] = o.q;
         }
       }
     };
     if (a.u) store(a.u);
     if (a.pre != FLETCHER_NORM_NONE) {
-      norm_row<VEC, NV, WPR>(v, a.pre, a.pre_gamma, a.pre_beta, a.eps, t, nvec, a.cols, red, turn);
+      norm_row<VEC, NV, WPR, FULL>(v, a.pre, a.pre_gamma, a.pre_beta, a.eps, t, nvec, a.cols, red, turn);
       store(a.h);
     }
   }
@@ -372,14 +395,16 @@ __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs 
   }
 }
 
-template <typename T, int VEC, int NV, int WPR, bool COMBINE>
+template <typename T, int VEC, int NV, int WPR, bool COMBINE, bool FULL = false>
 int32_t launch_vec(Ctx* c, const NormArgs& a) {
+  if constexpr (!FULL && VEC * sizeof(T) == 16)
+    if (a.cols == NV * VEC * WPR * 32) return launch_vec<T, VEC, NV, WPR, COMBINE, true>(c, a);
   constexpr int TEAMS = kThreads / (32 * WPR);
   // As few teams as walk the rows in the same number of turns.
   const int64_t most = (int64_t)c->num_sms * kMinBlocks<VEC, NV> * TEAMS;
   const int64_t turns = (a.rows + most - 1) / most;
   const int64_t blocks = (a.rows + turns * TEAMS - 1) / (turns * TEAMS);
-  FL_CUDA(c, launch_pdl(k_block_norm<T, VEC, NV, WPR, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
+  FL_CUDA(c, launch_pdl(k_block_norm<T, VEC, NV, WPR, FULL, COMBINE>, dim3((unsigned)blocks), dim3(kThreads), 0, c->stream, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
 }
