@@ -301,8 +301,9 @@ enum { FLETCHER_ROWS_TOKENS = 0, FLETCHER_ROWS_SLOTS = 1 };
  *   result[s] = act(input[row of s] . weight[e] + bias[e]),
  * weight [num_experts * inCols, outCols] (each expert's (in, out) matrix below the one before),
  * bias [num_experts, outCols] or NULL, result [slots, outCols], or outCols/2 columns for SwiGLU
- * (silu(first half) * second half).  act: IDENTITY, GELU, TANH or SWIGLU.  Sums are fp32.  `result`
- * must hold rows*top_k rows; those behind the last slot are left as they were.  inCols and outCols
+ * (silu(first half) * second half).  act: IDENTITY, GELU, TANH or SWIGLU.  Sums are fp32; `result`
+ * has the input's dtype, or f32, which keeps what Cuda_Combine_Grouped sums unrounded.  It must hold
+ * rows*top_k rows; those behind the last slot are left as they were.  inCols and outCols
  * are at most 2^24.  16-bit products whose inCols and output width are multiples of 8 and whose
  * buffers are 16-byte aligned run on the tensor cores, straight from the (in, out) weights;
  * others (and f32) on the fp32 units. */
@@ -333,7 +334,8 @@ typedef struct FletcherBlockNorm {
  * `rows` rows.  cols <= 49152. */
 int32_t Cuda_BlockNorm(CudaContextRef ctx, CudaBufferRef y, int64_t rows, int64_t cols,
                        const FletcherBlockNorm* norm, CudaBufferRef outResidual, CudaBufferRef outNorm);
-/* Joins the experts' outputs (grouped [slots, cols], as Cuda_Linear_Grouped wrote them):
+/* Joins the experts' outputs (grouped [slots, cols], as Cuda_Linear_Grouped wrote them, in the other
+ * buffers' dtype or f32):
  *   y[r] = sum over the row's choices that have a slot, in order, of weight * grouped[slot]
  * in fp32, followed by Cuda_BlockNorm's u and h of y; norm NULL means u = y.  An output may be the
  * same buffer as the residual or as a gate of `rows` rows, not as `grouped`. */

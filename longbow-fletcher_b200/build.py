@@ -22,7 +22,7 @@ FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", 
          "--expt-relaxed-constexpr", "-DFLETCHER_BUILD"]
 SOURCES = ["context.cu", "ops.cu", "gemm_simt.cu", "gemm_tc.cu", "attention.cu", "model.cu", "abi_ops.cu",
            "noalloc.cu", "attention_tc.cu", "probe.cu", "runtime.cu", "routing.cu",
-           "grouped_tc.cu", "grouped_simt.cu", "grouped_abi.cu", "block_norm.cu"]
+           "grouped_tc.cu", "grouped_simt.cu", "grouped_abi.cu", "block_norm.cu", "combine.cu"]
 
 
 def _deps():

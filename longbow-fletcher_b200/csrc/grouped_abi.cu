@@ -18,7 +18,8 @@ int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t
   FL_CHECK(c, r->rows >= 0, "Linear_Grouped: nothing routed yet");
   FL_CHECK(c, x && w && y, "Linear_Grouped: null buffer");
   const int32_t dt = x->dtype;
-  FL_CHECK(c, w->dtype == dt && y->dtype == dt && (!b || b->dtype == dt), "Linear_Grouped: dtype mismatch");
+  FL_CHECK(c, w->dtype == dt && (y->dtype == dt || y->dtype == FLETCHER_F32) && (!b || b->dtype == dt),
+           "Linear_Grouped: dtype mismatch");
   FL_CHECK(c, inputOrder == FLETCHER_ROWS_TOKENS || inputOrder == FLETCHER_ROWS_SLOTS,
            "Linear_Grouped: unknown input order %d", inputOrder);
   FL_CHECK(c, activation == FLETCHER_ACT_IDENTITY || activation == FLETCHER_ACT_GELU || activation == FLETCHER_ACT_TANH ||
@@ -46,7 +47,7 @@ int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t
            (long long)outCols);
   FL_CHECK(c, holds(c, y, a.pairs * a.n_out), "Linear_Grouped: result must hold %lldx%lld", (long long)a.pairs,
            (long long)a.n_out);
-  const int64_t es = dtype_size(dt), ybytes = a.pairs * a.n_out * es;
+  const int64_t es = dtype_size(dt), ybytes = a.pairs * a.n_out * dtype_size(y->dtype);
   FL_CHECK(c, !overlap(y->ptr, ybytes, x->ptr, a.x_rows * inCols * es) &&
                   !overlap(y->ptr, ybytes, w->ptr, a.experts * inCols * outCols * es) &&
                   !(b && overlap(y->ptr, ybytes, b->ptr, a.experts * outCols * es)) &&
@@ -61,6 +62,7 @@ int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t
   a.slots = inputOrder == FLETCHER_ROWS_TOKENS ? r->slots : nullptr;
   a.pair_of = inputOrder == FLETCHER_ROWS_TOKENS ? r->pair_of : nullptr;
   a.act = activation;
+  a.out32 = dt != FLETCHER_F32 && y->dtype == FLETCHER_F32;
   if (grouped_tc_supported(dt, a)) {
     void* ws = nullptr;
     const int64_t need = grouped_tc_workspace(a);

@@ -179,7 +179,10 @@ __global__ void __launch_bounds__((BM / TM) * (BN / TN) * KS) k_grouped_simt(con
       } else {
         v = act1<T, ACT>(v);
       }
-      out[s * a.n_out + n] = from_f<T>(v);
+      if (a.out32)
+        reinterpret_cast<float*>(a.out)[s * a.n_out + n] = v;
+      else
+        out[s * a.n_out + n] = from_f<T>(v);
     }
   }
 }

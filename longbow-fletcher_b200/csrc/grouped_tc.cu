@@ -74,6 +74,7 @@ struct Args {
   int32_t* err;
   int64_t N, n_out;
   int32_t E, top_k, num_kb, n_tiles, act;
+  int32_t out32;  // fp32 result: 1, or 2 where its rows are 32-byte aligned
 };
 
 template <bool PAIR>
@@ -173,10 +174,35 @@ __device__ __forceinline__ float silu16(float g) { return __fdividef(g, 1.0f + _
 
 __device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 
-// Row-per-lane 64 values -> 16-byte chunks of T.
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
+// A lane's N values of a row, columns col.. of n_out, from registers.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const Args& args, const float* v, int64_t row, int64_t col) {
+  if (args.out32) {
+    float* dst = reinterpret_cast<float*>(args.out) + row * args.n_out + col;
+#pragma unroll
+    for (int j = 0; j < N; j += 8) {
+      if (col + j < args.n_out) {
+        if (args.out32 == 2) {  // whole 32-byte sectors
+          asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + j), "f"(v[j]), "f"(v[j + 1]),
+                       "f"(v[j + 2]), "f"(v[j + 3]), "f"(v[j + 4]), "f"(v[j + 5]), "f"(v[j + 6]), "f"(v[j + 7])
+                       : "memory");
+        } else {
+          reinterpret_cast<float4*>(dst + j)[0] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          reinterpret_cast<float4*>(dst + j)[1] = make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
+        }
+      }
+    }
+  } else {
+    T* dst = reinterpret_cast<T*>(args.out) + row * args.n_out + col;
+#pragma unroll
+    for (int j = 0; j < N; j += 8)
+      if (col + j < args.n_out) *reinterpret_cast<uint4*>(dst + j) = pack8<T>(v + j);
+  }
 }
 
 // Persistent: warp 0 loads by TMA, warp 1 issues the MMAs and owns the TMEM, warps 2-9 drain one
@@ -340,7 +366,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int UW = OUT_N >= 128 ? 64 : 32, UNITS = OUT_N / 2 / UW;  // a warp's units of UW columns
     uint8_t* box = smem + C::OUT_OFF + (warp - 2) * kBox;
     const uint32_t tempty_lead = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0;
-    T* out = reinterpret_cast<T*>(args.out);
     int it = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_stride, ++it) {
       const Tile t = walk.at(tile);
@@ -397,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (ocol >= args.n_out || row0 >= t.end) continue;
-        if (UW == 64 && row0 + 32 <= t.end) {
+        if (UW == 64 && row0 + 32 <= t.end && !args.out32) {
           // 32 whole rows: staged in the swizzled box and stored by TMA, columns past the end clipped.
           if (lane == 0) bulk_wait_read0();  // the box's last store has left it
           __syncwarp();
@@ -410,11 +435,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_store_2d(&tmC, box, (int)ocol, row0);
             bulk_commit();
           }
-        } else if (row0 + lane < t.end) {  // the group's last rows: the next rows are another group's
-          T* dst = out + (int64_t)(row0 + lane) * args.n_out + ocol;
-#pragma unroll
-          for (int j = 0; j < UW / 8; j++)
-            if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
+        } else if (row0 + lane < t.end) {  // the group's last rows (the next are another group's), or fp32
+          store_row<T, UW>(args, v, row0 + lane, ocol);
         }
       }
     }
@@ -627,12 +649,7 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
 #pragma unroll
       for (int i = 0; i < 64; i += 2) gelu_pair(v[i], v[i + 1]);
     }
-    if (t.first + lane < t.end) {
-      T* dst = reinterpret_cast<T*>(args.out) + (int64_t)(t.first + lane) * args.n_out + ocol;
-#pragma unroll
-      for (int j = 0; j < COLS / 8; j++)
-        if (ocol + 8 * j < args.n_out) reinterpret_cast<uint4*>(dst)[j] = pack8<T>(v + 8 * j);
-    }
+    if (t.first + lane < t.end) store_row<T, COLS>(args, v, t.first + lane, ocol);
   };
   if (!SPLIT && (warp == 0 || warp == 4)) {
     int it = 0;
@@ -719,6 +736,7 @@ Args args_of(const Ctx* c, const GroupedArgs& g, int out_n) {
   a.num_kb = (int)((g.K + BK - 1) / BK);
   a.n_tiles = (int)((g.n_out + out_n - 1) / out_n);
   a.act = g.act;
+  a.out32 = !g.out32 ? 0 : ((uintptr_t)g.out & 31) == 0 ? 2 : 1;
   return a;
 }
 
@@ -790,7 +808,9 @@ int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
   if ((rc = make_tma_map_2d(c, &ma, dt, g.x, (uint64_t)g.x_rows, (uint64_t)g.K, (uint64_t)g.K, BK, BM)))
     return rc;
   if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
-  if ((rc = make_tma_map_2d(c, &mc, dt, g.out, (uint64_t)g.pairs, (uint64_t)g.n_out, (uint64_t)g.n_out, 64, 32)))
+  mc = ma;  // not used for an fp32 result
+  if (!g.out32 &&
+      (rc = make_tma_map_2d(c, &mc, dt, g.out, (uint64_t)g.pairs, (uint64_t)g.n_out, (uint64_t)g.n_out, 64, 32)))
     return rc;
   const Args a = args_of(c, g, OUT_N);
   auto kern = k_grouped_tc<T, BN, PAIR, GATED>;

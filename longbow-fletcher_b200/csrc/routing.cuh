@@ -62,6 +62,7 @@ struct GroupedArgs {
   int32_t top_k, experts;
   int64_t pairs;  // upper bound of the slots
   int32_t act;
+  bool out32;  // 16-bit operands, fp32 result
 };
 bool grouped_tc_supported(int32_t dtype, const GroupedArgs& a);
 int64_t grouped_tc_workspace(const GroupedArgs& a);  // bytes

@@ -449,11 +449,12 @@ class BlockNorm:
                 raise FletcherError(1, f"BlockNorm: {name} has {t.rows} rows, {need} are needed")
         return self._p
 
-    def _outputs(self, y, rows, out, out_norm):
+    def _outputs(self, y, rows, out, out_norm, combine=False):
         if out is None and out_norm is None:
-            out = Tensor(y.be, rows, y.cols, y.dtype)
+            like = (self._tensors["residual"] or self._tensors["gate"] or y) if combine else y
+            out = Tensor(y.be, rows, y.cols, like.dtype)
             if self.c.pre_kind != NORM_NONE:
-                out_norm = Tensor(y.be, rows, y.cols, y.dtype)
+                out_norm = Tensor(y.be, rows, y.cols, like.dtype)
         return out, out_norm
 
 
@@ -503,24 +504,27 @@ class Routing:
         self.be.check(lib().Cuda_Routing_DevicePointers(self.h, *(ctypes.byref(x) for x in p)))
         return dict(zip(("experts", "weights", "slots", "offsets"), (x.value for x in p)))
 
-    def linear(self, x: Tensor, w: Tensor, b: "Tensor | None" = None, act=ACT_IDENTITY, grouped_input=False, out=None):
+    def linear(self, x: Tensor, w: Tensor, b: "Tensor | None" = None, act=ACT_IDENTITY, grouped_input=False, out=None,
+               dtype=None):
         """Cuda_Linear_Grouped: w (num_experts * in, out), b (num_experts, out); one output row a slot.
-        x holds one row a token, or with grouped_input one row a slot."""
+        x holds one row a token, or with grouped_input one row a slot.  The result has x's dtype, or F32."""
         if w.rows != self.num_experts * x.cols:
             raise FletcherError(1, f"Linear_Grouped: weight has {w.rows} rows, not {self.num_experts} x {x.cols}")
-        y = out or Tensor(self.be, self.rows * self.top_k, w.cols // 2 if act == ACT_SWIGLU else w.cols, x.dtype)
+        y = out or Tensor(self.be, self.rows * self.top_k, w.cols // 2 if act == ACT_SWIGLU else w.cols,
+                          x.dtype if dtype is None else dtype)
         self.be.check(lib().Cuda_Linear_Grouped(self.h, x.buf, ROWS_SLOTS if grouped_input else ROWS_TOKENS, x.cols,
                                                 w.buf, w.cols, b.buf if b is not None else None, y.buf, act))
         return y
 
     def combine(self, grouped: Tensor, norm: "BlockNorm | None" = None, out=None, out_norm=None):
         """Cuda_Combine_Grouped: the weighted sum of each row's slots, then the norm's u and h.
-        Without a norm returns the sum, else (u, h) as Tensor.block_norm does."""
+        Without a norm returns the sum, else (u, h) as Tensor.block_norm does; tensors that are made have
+        the residual's dtype, else the gate's, else grouped's."""
         if norm is None:
             out = out or Tensor(self.be, self.rows, grouped.cols, grouped.dtype)
             self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, None, out.buf, None))
             return out
-        out, out_norm = norm._outputs(grouped, self.rows, out, out_norm)
+        out, out_norm = norm._outputs(grouped, self.rows, out, out_norm, combine=True)
         self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, norm._ref(self.rows),
                                                  out.buf if out else None, out_norm.buf if out_norm else None))
         return out, out_norm

@@ -218,7 +218,8 @@ def test_routing_assign(fl, be, rows, experts, k):
 
 
 # ---------------------------------------------------------------- grouped products
-def run_grouped(fl, be, rows, experts, k, K, N, act, dtype, bias, grouped_input, ids=None, seed=0):
+def run_grouped(fl, be, rows, experts, k, K, N, act, dtype, bias, grouped_input, ids=None, seed=0, out=None):
+    out = out or dtype
     rng = np.random.default_rng(seed + rows + 7 * K + 13 * N)
     if ids is None:
         ids = np.argsort(rng.random((rows, experts)) + np.linspace(0, 1, experts), 1)[:, :k].astype(np.int32)
@@ -229,8 +230,8 @@ def run_grouped(fl, be, rows, experts, k, K, N, act, dtype, bias, grouped_input,
     r = be.routing(rows + 5, experts, k)
     r.assign(ids)
     n_out = N // 2 if act == 4 else N
-    before = quantise(rng.standard_normal((pairs + 2, n_out)), dtype)  # rows behind the last stay
-    y = tensor(fl, be, before, dtype)
+    before = quantise(rng.standard_normal((pairs + 2, n_out)), out)  # rows behind the last stay
+    y = tensor(fl, be, before, out)
     r.linear(tensor(fl, be, x, dtype), tensor(fl, be, w, dtype), None if b is None else tensor(fl, be, b, dtype), act,
              grouped_input, out=y)
     got = y.to_host()
@@ -238,7 +239,7 @@ def run_grouped(fl, be, rows, experts, k, K, N, act, dtype, bias, grouped_input,
     want, tol, skip = grouped_ref(x, w, b, ids, experts, act, grouped_input)
     n = want.shape[0]
     assert (got[n:] == before[n:]).all(), "rows behind the last slot were written"
-    check(np.where(skip, want, got[:n]), want, tol, dtype, f"{rows} {experts} {k} {K} {N} {act} {dtype}")
+    check(np.where(skip, want, got[:n]), want, tol, out, f"{rows} {experts} {k} {K} {N} {act} {dtype}")
 
 
 SHAPES = [  # rows, experts, k, K, N
@@ -253,6 +254,14 @@ SHAPES = [  # rows, experts, k, K, N
 def test_linear_grouped(fl, be, rows, experts, k, K, N, act, dtype):
     run_grouped(fl, be, rows, experts, k, K, N, act, dtype, act != 0, False)
     run_grouped(fl, be, rows, experts, k, K, N, act, dtype, act == 0, True)
+
+
+@pytest.mark.parametrize("rows,experts,k,K,N", [SHAPES[i] for i in (0, 3, 4, 7, 8, 9)] + [(70, 3, 2, 17, 66), (2100, 3, 1, 64, 776)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_linear_grouped_f32_result(fl, be, rows, experts, k, K, N, dtype):
+    """16-bit operands, the sums kept in fp32."""
+    for act in (0, 1, 4):
+        run_grouped(fl, be, rows, experts, k, K, N, act, dtype, act == 1, act == 0, out="f32")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
@@ -379,21 +388,22 @@ def test_block_norm_in_place(fl, be, dtype, cols):
         assert (t[u_over].to_host() == wu).all() and (t[h_over].to_host() == wh).all()
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("dtype,slots_dtype", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("bf16", "f32"), ("f16", "f32")])
 @pytest.mark.parametrize("rows,experts,k,cols", [(1, 8, 2, 768), (40, 4, 1, 8), (257, 16, 5, 100), (600, 8, 2, 1536),
                                                  (33, 3, 3, 2049), (5, 4, 4, 8192)])
-def test_combine(fl, be, rows, experts, k, cols, dtype):
+def test_combine(fl, be, rows, experts, k, cols, dtype, slots_dtype):
     rng = np.random.default_rng(rows + cols)
     ids = rng.integers(-1, experts, (rows, k)).astype(np.int32)
     w = rng.standard_normal((rows, k)).astype(np.float32)
     r = be.routing(rows, experts, k)
     r.assign(ids, w)
     slots = group_ref(ids, experts)[0]
-    g = quantise(rng.standard_normal((rows * k, cols)), dtype)
-    tg = tensor(fl, be, g, dtype)
+    g = quantise(rng.standard_normal((rows * k, cols)), slots_dtype)
+    tg = tensor(fl, be, g, slots_dtype)
     terms = np.where(slots[..., None] >= 0, w[..., None] * g.astype(np.float64)[np.maximum(slots, 0)], 0.0)
     y, mag = terms.sum(1), np.abs(terms).sum(1)
-    check(r.combine(tg).to_host(), y, (k + 1) * E24 * mag, dtype)
+    plain = be.new_tensor(rows, cols, None, fl.DTYPES[dtype])
+    check(r.combine(tg, out=plain).to_host(), y, (k + 1) * E24 * mag, dtype)
     c = norm_case(rng, rows, cols, dtype, 0, 1, 1, True)
     norm, t = make_norm(fl, be, c, dtype, 0, 1, 1e-5, 1.0, 1.0)
     u, h, eu, eh = norm_expect(c, y, 0, 1, 1e-5, 1.0, 1.0)
@@ -439,7 +449,7 @@ def test_expert_block(fl, be, rows, experts, k, H, I, act, dtype):
     t["norm"] = fl.BlockNorm(pre=fl.NORM_LAYER, eps=1e-5, residual=t["x"])
     r = be.routing(rows, experts, k)
     dt = fl.DTYPES[dtype]
-    mid, out2, out = (be.new_tensor(n, m, None, dt) for n, m in ((rows * k, I), (rows * k, H), (rows, H)))
+    mid, out2, out = (be.new_tensor(n, m, None, d) for n, m, d in ((rows * k, I, dt), (rows * k, H, fl.F32), (rows, H, dt)))
     block(be, fl, r, t, mid, out2, out, act)
     got = out.to_host()
     ids, w = route_ref(a["logits"], k)
@@ -447,8 +457,8 @@ def test_expert_block(fl, be, rows, experts, k, H, I, act, dtype):
     h, _, _ = grouped_ref(a["x"], a["up"], None, ids, experts, act, False)
     g, _, _ = grouped_ref(h, a["down"], None, ids, experts, 0, True)
     want = norm_ref(a["x"] + (w[..., None] * g[slots]).sum(1), 1, None, None, 1e-5)
-    # Three roundings to T meet (h, the experts' outputs, the result), each of relative size u on
-    # values whose rows have a norm of at most a few times the result's: 6 u of a row's norm.
+    # Two roundings to T meet (h and the result; the experts' outputs stay fp32), each of relative size u
+    # on values whose rows have a norm of at most a few times the result's: 6 u of a row's norm.
     err = np.linalg.norm(got - want, axis=1) / np.linalg.norm(want, axis=1)
     assert err.max() <= (6 * U[dtype] if dtype != "f32" else 2e-5), err.max()
 
@@ -546,6 +556,8 @@ def test_refusals(fl, be):
     assert L.Cuda_Linear_Grouped(r.h, None, 0, 16, w.buf, 32, None, y.buf, 0) == 1
     assert L.Cuda_Linear_Grouped(None, x.buf, 0, 16, w.buf, 32, None, y.buf, 0) == 1
     refuses(fl, be, lambda: r.combine(g, out=g), "overlaps")
+    refuses(fl, be, lambda: r.combine(g, out=new(8, 16, "f16")), "dtype")
+    refuses(fl, be, lambda: new(8, 16, "f32").block_norm(fl.BlockNorm(), out=new(8, 16)), "dtype")
     refuses(fl, be, lambda: r.combine(g, out=new(7, 16)), "outputs must be")
     refuses(fl, be, lambda: r.combine(new(15, 16), out=new(8, 16)), "input must hold")
 
