@@ -374,7 +374,7 @@ def _handles(s):
     if c["op"] == "layer":
         pairs = c["rows"] * c["k"]
         h["mid"] = be.new_tensor(pairs, c["inner"], None, dt)
-        h["expert_out"] = be.new_tensor(pairs, c["hidden"], None, dt)
+        h["expert_out"] = be.new_tensor(pairs, c["hidden"], None, fl.F32)  # summed before they are rounded
     if c["op"] == "blocknorm":
         h["norm"] = fl.BlockNorm(post=NORMS[c["post"]], pre=NORMS[c["pre"]], eps=EPS, residual=h["residual"],
                                  gate=h["gate"], residual_scale=c["residual_scale"], post_gamma=h["post_gamma"],
