@@ -377,7 +377,8 @@ def _handles(s):
         h["expert_out"] = be.new_tensor(pairs, c["hidden"], None, fl.F32)  # summed before they are rounded
     if c["op"] == "blocknorm":
         h["norm"] = fl.BlockNorm(post=NORMS[c["post"]], pre=NORMS[c["pre"]], eps=EPS, residual=h["residual"],
-                                 gate=h["gate"], residual_scale=c["residual_scale"], post_gamma=h["post_gamma"],
+                                 gate=h["gate"], residual_scale=c["residual_scale"],
+                                 post_gamma=h["post_gamma"] if c["post"] != "none" else None,
                                  post_beta=h["post_beta"] if c["post"] == "layer" else None, pre_gamma=h["pre_gamma"],
                                  pre_beta=h["pre_beta"] if c["pre"] == "layer" else None)
     elif c["op"] == "layer" or c.get("norm", "none") != "none":
