@@ -129,8 +129,8 @@ int32_t Cuda_SetHalfConversion(CudaContextRef ctx, int32_t mode);
 CudaBufferRef Cuda_Alloc(CudaContextRef ctx, int64_t size);
 CudaBufferRef Cuda_AllocTensor(CudaContextRef ctx, int64_t rows, int64_t cols, int32_t dtype);
 /* A buffer over device memory that the caller owns (a host framework's tensor): rows*cols dense
- * elements of dtype at `ptr`, which must be memory of the context's device, aligned to the element
- * size, and outlive the buffer; Cuda_FreeBuffer releases the handle alone.  The caller orders its
+ * elements of dtype at `ptr`, which must be memory of the context's device, aligned to 32 bytes, and
+ * outlive the buffer; Cuda_FreeBuffer releases the handle alone.  The caller orders its
  * own streams with the context's (Cuda_GetStream, Cuda_Synchronize).  As the contents can change
  * behind this ABI, Cuda_Linear_Fused lays such a weight out anew in every call.  NULL on error.
  * (No counterpart in the reference.) */
@@ -265,7 +265,7 @@ int32_t Cuda_MeanPoolL2(CudaContextRef ctx, CudaBufferRef hidden, const int32_t*
  * weights, and the order of the choices by expert.  Choice j of row r is pair r*top_k + j; pairs
  * sorted by expert, then by pair, are given the slots 0, 1, ...; expert e owns the slots
  * [offsets[e], offsets[e+1]).  A choice of -1 has no slot.  1 <= num_experts <= 256,
- * 1 <= top_k <= min(16, num_experts), max_rows * top_k < 2^31.
+ * 1 <= top_k <= min(16, num_experts), max_rows * top_k <= 2^30.
  * A routing's device memory belongs to its context (as a buffer's does): free it before the
  * context.  The next Cuda_Routing_TopK or Assign overwrites it in stream order; graphs that share
  * one routing must not run at the same time. */
@@ -304,9 +304,8 @@ enum { FLETCHER_ROWS_TOKENS = 0, FLETCHER_ROWS_SLOTS = 1 };
  * (silu(first half) * second half).  act: IDENTITY, GELU, TANH or SWIGLU.  Sums are fp32; `result`
  * has the input's dtype, or f32, which keeps what Cuda_Combine_Grouped sums unrounded.  It must hold
  * rows*top_k rows; those behind the last slot are left as they were.  inCols and outCols
- * are at most 2^24.  16-bit products whose inCols and output width are multiples of 8 and whose
- * buffers are 16-byte aligned run on the tensor cores, straight from the (in, out) weights;
- * others (and f32) on the fp32 units. */
+ * are at most 2^24.  16-bit products whose inCols and output width are multiples of 8 run on the
+ * tensor cores, straight from the (in, out) weights; others (and f32, and TANH) on the fp32 units. */
 int32_t Cuda_Linear_Grouped(CudaRoutingRef routing, CudaBufferRef input, int32_t inputOrder, int64_t inCols,
                             CudaBufferRef weight, int64_t outCols, CudaBufferRef bias, CudaBufferRef result,
                             int32_t activation);

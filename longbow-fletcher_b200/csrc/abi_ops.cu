@@ -43,17 +43,19 @@ int32_t upload(Ctx* c, Temp& t, const void* h, int64_t bytes) {
 int32_t packed_weight(Ctx* c, Buf* w, int64_t K, int64_t N, bool swiglu, int bn, const void** out) {
   const int key = (swiglu ? 1 : 0) | (bn << 1);
   const int64_t bytes = K * N * 2;
-  if (!(!w->external && w->packed && w->packed_key == key && w->packed_ver == w->version && w->packed_bytes == bytes)) {
+  int32_t rc;
+  if (!(w->packed && w->packed_bytes == bytes)) {
     dev_free(c, w->packed, w->packed_bytes);
     w->packed = nullptr;
     w->packed_bytes = 0;
-    int32_t rc = dev_alloc(c, &w->packed, bytes);
-    if (rc) return rc;
+    w->packed_key = -1;
+    if ((rc = dev_alloc(c, &w->packed, bytes))) return rc;
     w->packed_bytes = bytes;
-    if ((rc = launch_pack_kmajor_16(c, w->dtype, w->ptr, K, N, w->packed, swiglu ? 1 : 0, bn))) {
-      w->packed_key = -1;
-      return rc;
-    }
+  }
+  // A wrapped weight (the caller's memory) may have changed unseen: laid out in every call.
+  if (w->external || w->packed_key != key || w->packed_ver != w->version) {
+    w->packed_key = -1;
+    if ((rc = launch_pack_kmajor_16(c, w->dtype, w->ptr, K, N, w->packed, swiglu ? 1 : 0, bn))) return rc;
     w->packed_key = key;
     w->packed_ver = w->version;
   }
@@ -64,13 +66,16 @@ int32_t packed_weight(Ctx* c, Buf* w, int64_t K, int64_t N, bool swiglu, int bn,
 // The bias widened to fp32 in the packed column order, cached like the weight.
 int32_t packed_bias(Ctx* c, Buf* b, int64_t N, bool swiglu, int bn, const float** out) {
   const int key = (swiglu ? 1 : 0) | (bn << 1);
-  if (!(!b->external && b->bias32 && b->bias32_key == key && b->bias32_ver == b->version && b->bias32_bytes == N * 4)) {
+  int32_t rc;
+  if (!(b->bias32 && b->bias32_bytes == N * 4)) {
     dev_free(c, b->bias32, b->bias32_bytes);
     b->bias32 = nullptr;
     b->bias32_bytes = 0;
-    int32_t rc = dev_alloc(c, (void**)&b->bias32, N * 4);
-    if (rc) return rc;
+    b->bias32_key = -1;
+    if ((rc = dev_alloc(c, (void**)&b->bias32, N * 4))) return rc;
     b->bias32_bytes = N * 4;
+  }
+  if (b->external || b->bias32_key != key || b->bias32_ver != b->version) {
     b->bias32_key = -1;
     if (swiglu) {  // interleave the bias like the weight rows: pack a [1, N] row as K=1
       Temp b16(c);

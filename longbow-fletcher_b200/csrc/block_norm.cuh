@@ -38,7 +38,7 @@ struct NormArgs {
   int32_t cols;
 };
 
-// VEC elements moved at once: 16 bytes, or what a row's width and alignment allow.
+// VEC elements moved at once: 16 bytes, or what a row's width allows.
 template <int BYTES>
 struct RawOf;
 template <>
@@ -373,7 +373,7 @@ __device__ __forceinline__ void norm_generic(float* v, int kind, const float* ga
     v[c] = fmaf(v[c] * inv, gamma ? gamma[c] : 1.0f, beta ? beta[c] : 0.0f);
 }
 
-// Any width and alignment: a block per row, the row in shared memory, each column always with the
+// Any width: a block per row, the row in shared memory, each column always with the
 // same thread (so outputs may lie over inputs).
 template <typename T, typename TY, bool COMBINE>
 __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs a) {
@@ -438,11 +438,8 @@ constexpr int kNarrowMost = 16 * 256;
 template <typename T, typename TY, bool COMBINE>
 int32_t launch_norm(Ctx* c, const NormArgs& a) {
   constexpr int VEC = 16 / sizeof(T);
-  uintptr_t tensors = 0, tables = 0;
-  for (const void* p : {a.y, a.residual, a.gate, (const void*)a.u, (const void*)a.h}) tensors |= (uintptr_t)p;
-  for (const float* p : {a.post_gamma, a.post_beta, a.pre_gamma, a.pre_beta}) tables |= (uintptr_t)p;
   const int nvec = a.cols / VEC;
-  if (a.cols % VEC == 0 && ((tensors | tables) & 15) == 0 && nvec <= 1024) {
+  if (a.cols % VEC == 0 && nvec <= 1024) {
     // The fewest warps a row whose lanes hold at most four vectors each (two vectors in twice the warps:
     // 49152 x 1024 in 87 us against 79, 65536 x 768 in 102 against 80).
     if (nvec <= 32) return launch_vec<T, TY, VEC, 1, 1, COMBINE>(c, a);
@@ -457,7 +454,7 @@ int32_t launch_norm(Ctx* c, const NormArgs& a) {
     return launch_vec<T, TY, VEC, 4, 8, COMBINE>(c, a);
   }
   if constexpr (sizeof(T) == 2) {
-    if (a.cols % 2 == 0 && (tensors & 3) == 0 && a.cols <= 2 * kNarrowMost) return launch_narrow<T, TY, 2, COMBINE>(c, a);
+    if (a.cols % 2 == 0 && a.cols <= 2 * kNarrowMost) return launch_narrow<T, TY, 2, COMBINE>(c, a);
   }
   if (a.cols <= kNarrowMost) return launch_narrow<T, TY, 1, COMBINE>(c, a);
   auto kern = k_block_norm_generic<T, TY, COMBINE>;

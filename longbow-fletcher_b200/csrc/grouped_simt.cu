@@ -1,5 +1,5 @@
 // Grouped product on the fp32 units: f32 (the parity type) and the 16-bit shapes the tensor-core
-// kernels do not take (widths that 16 bytes do not divide, unaligned buffers, TANH).
+// kernels do not take (widths that 16 bytes do not divide, TANH).
 #include <algorithm>
 
 #include "routing.cuh"
@@ -51,7 +51,7 @@ __device__ __forceinline__ float act1(float v) {
 // One BM x BN output tile a block (SwiGLU: its gate and up columns), TM x TN sums a thread in packed pairs
 // along n, K in slabs of 16: the next slab's elements are on their way from memory while this one's are
 // multiplied from shared memory.  Rows are gathered as they are loaded; single elements, so that any
-// width and alignment does.  KS teams of threads take alternate slabs.  Bound by the fp32 units (34
+// width does.  KS teams of threads take alternate slabs.  Bound by the fp32 units (34
 // TFLOP/s at 4000 x 2 rows of 8 experts, 500 -> 500), for few rows by a slab's chain of load, store and
 // multiply, which teams overlap.
 template <typename T, int ACT, int BM, int BN, int TM, int TN, int KS>

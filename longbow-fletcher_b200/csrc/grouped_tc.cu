@@ -74,7 +74,7 @@ struct Args {
   int32_t* err;
   int64_t N, n_out;
   int32_t E, top_k, num_kb, n_tiles, act;
-  int32_t out32;  // fp32 result: 1, or 2 where its rows are 32-byte aligned
+  int32_t out32;  // fp32 result
 };
 
 template <bool PAIR>
@@ -186,16 +186,10 @@ __device__ __forceinline__ void store_row(const Args& args, const float* v, int6
     float* dst = reinterpret_cast<float*>(args.out) + row * args.n_out + col;
 #pragma unroll
     for (int j = 0; j < N; j += 8) {
-      if (col + j < args.n_out) {
-        if (args.out32 == 2) {  // whole 32-byte sectors
-          asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + j), "f"(v[j]), "f"(v[j + 1]),
-                       "f"(v[j + 2]), "f"(v[j + 3]), "f"(v[j + 4]), "f"(v[j + 5]), "f"(v[j + 6]), "f"(v[j + 7])
-                       : "memory");
-        } else {
-          reinterpret_cast<float4*>(dst + j)[0] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          reinterpret_cast<float4*>(dst + j)[1] = make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
-        }
-      }
+      if (col + j < args.n_out)  // whole 32-byte sectors
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + j), "f"(v[j]), "f"(v[j + 1]),
+                     "f"(v[j + 2]), "f"(v[j + 3]), "f"(v[j + 4]), "f"(v[j + 5]), "f"(v[j + 6]), "f"(v[j + 7])
+                     : "memory");
     }
   } else {
     T* dst = reinterpret_cast<T*>(args.out) + row * args.n_out + col;
@@ -736,7 +730,7 @@ Args args_of(const Ctx* c, const GroupedArgs& g, int out_n) {
   a.num_kb = (int)((g.K + BK - 1) / BK);
   a.n_tiles = (int)((g.n_out + out_n - 1) / out_n);
   a.act = g.act;
-  a.out32 = !g.out32 ? 0 : ((uintptr_t)g.out & 31) == 0 ? 2 : 1;
+  a.out32 = g.out32;
   return a;
 }
 
@@ -891,8 +885,7 @@ int32_t launch(Ctx* c, int32_t dt, const GroupedArgs& g) {
 }  // namespace tcg
 
 bool grouped_tc_supported(int32_t dtype, const GroupedArgs& g) {
-  const uintptr_t ptrs = (uintptr_t)g.x | (uintptr_t)g.w | (uintptr_t)g.bias | (uintptr_t)g.out;
-  return dtype != FLETCHER_F32 && (ptrs & 15) == 0 && g.K % 8 == 0 && g.n_out % 8 == 0 && g.act != FLETCHER_ACT_TANH;
+  return dtype != FLETCHER_F32 && g.K % 8 == 0 && g.n_out % 8 == 0 && g.act != FLETCHER_ACT_TANH;
 }
 
 // Rows an expert on average, counting no more experts than there are rows, decide between the kernels.

@@ -136,7 +136,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
   const int lane = threadIdx.x & 31, gl = lane & (L - 1);
   const int chunks = (a.E + V * L - 1) / (V * L);
   const T* z = reinterpret_cast<const T*>(a.logits);
-  const bool vec = a.E % V == 0 && ((uintptr_t)z & 15) == 0;
+  const bool vec = a.E % V == 0;
   struct alignas(16) Chunk {
     T t[V];
   };
@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
   if constexpr (ONE) {
     __shared__ int32_t all[kMaxExperts], before[kMaxExperts];
     const bool cluster = gridDim.x > 1;  // the grid is the cluster
+    __syncwarp();
     if (cluster)
       asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     else
@@ -393,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
       all[e] = n;
       before[e] = b;
     }
+    __syncwarp();
     if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' counts are read
     __syncthreads();
     const int32_t total = scan_experts(all, at, a.E, tmp);
@@ -404,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
     for (int e = threadIdx.x; e < a.E; e += kThreads) at[e] += before[e];
     __syncthreads();
     if (r0 < r1) assign_slots(a, r0 * a.k, (int)((r1 - r0) * a.k), ids, at, dyn);
+    __syncwarp();
     if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody reads this block's now
   } else {
     __syncthreads();
@@ -611,7 +614,7 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
            kMaxExperts);
   FL_CHECK(c, top_k >= 1 && top_k <= std::min(kMaxTopK, num_experts), "Routing: %d choices outside [1, %d]", top_k,
            std::min(kMaxTopK, num_experts));
-  FL_CHECK(c, max_rows >= 0 && max_rows <= (int64_t)INT32_MAX / top_k, "Routing: %lld rows are too many",
+  FL_CHECK(c, max_rows >= 0 && max_rows <= ((int64_t)1 << 30) / top_k, "Routing: %lld rows are too many",
            (long long)max_rows);
   Routing* r = new (std::nothrow) Routing();
   if (!r) return set_error(c, FLETCHER_ERR_OOM, "Routing: out of host memory");
@@ -661,6 +664,8 @@ int32_t Cuda_Routing_TopK(CudaRoutingRef routing, CudaBufferRef logits, int64_t 
            (long long)r->max_rows);
   FL_CHECK(c, holds(c, z, rows * r->num_experts), "Routing: logits must hold %lldx%d on the context's device",
            (long long)rows, r->num_experts);
+  FL_CHECK(c, !overlap(z->ptr, rows * r->num_experts * dtype_size(z->dtype), r->mem, r->bytes),
+           "Routing: the logits overlap the routing");
   FL_CHECK(c, scoring == FLETCHER_SCORE_SOFTMAX || scoring == FLETCHER_SCORE_SIGMOID, "Routing: unknown scoring %d",
            scoring);
   RouteArgs a{};

@@ -172,6 +172,19 @@ def test_routing(fl, be, rows, experts, k, dtype):
         assert (got["slots"] == slots).all() and (got["offsets"] == offsets).all()
 
 
+@pytest.mark.parametrize("rows,experts,k,dtype", [(300000, 16, 8, "bf16"), (200003, 5, 1, "f32")])
+def test_routing_many_rows(fl, be, rows, experts, k, dtype):
+    """More pairs a block than it ranks at once, and as many blocks as there are."""
+    rng = np.random.default_rng(rows)
+    z = quantise(rng.standard_normal((rows, experts)) + np.linspace(0, 2, experts), dtype)
+    r = be.routing(rows, experts, k)
+    r.route(tensor(fl, be, z, dtype))
+    got = r.read()
+    ids, _ = route_ref(z, k)
+    slots, offsets, _ = group_ref(ids, experts)
+    assert (got["experts"] == ids).all() and (got["slots"] == slots).all() and (got["offsets"] == offsets).all()
+
+
 def test_routing_masks(fl, be):
     inf, nan, low = np.inf, np.nan, float(np.finfo(np.float32).min)
     z = np.array([[-inf] * 4, [nan] * 4, [0, -inf, nan, -inf], [inf, 1, inf, 0], [low] * 4, [low, 0, low, -inf],
@@ -186,20 +199,6 @@ def test_routing_masks(fl, be):
             assert np.allclose(got["weights"], w, rtol=1e-5, atol=0)
             slots, offsets, _ = group_ref(ids, 4)
             assert (got["slots"] == slots).all() and (got["offsets"] == offsets).all()
-
-
-def test_routing_unaligned_logits(fl, be):
-    """Logits whose rows start off a 16-byte boundary (a wrapped tensor at an odd element)."""
-    import torch
-    rng = np.random.default_rng(5)
-    z = rng.standard_normal((40, 16)).astype(np.float32)
-    flat = torch.zeros(40 * 16 + 1, device="cuda")
-    flat[1:] = torch.from_numpy(z.reshape(-1)).cuda()
-    torch.cuda.synchronize()
-    t = be.wrap(flat.data_ptr() + 4, 40, 16, fl.F32)
-    r = be.routing(40, 16, 4)
-    r.route(t)
-    assert (r.read()["experts"] == route_ref(z, 4)[0]).all()
 
 
 @pytest.mark.parametrize("rows,experts,k", [(5, 4, 2), (3000, 7, 3), (20000, 256, 2)])
@@ -526,7 +525,7 @@ def refuses(fl, be, call, text):
 def test_refusals(fl, be):
     L = fl.lib()
     new = lambda r, c, dt="bf16": be.new_tensor(r, c, None, fl.DTYPES[dt])  # noqa: E731
-    for rows, experts, k in ((-1, 8, 2), (4, 0, 1), (4, 257, 1), (4, 8, 0), (4, 8, 9), (4, 64, 17), (1 << 30, 8, 2)):
+    for rows, experts, k in ((-1, 8, 2), (4, 0, 1), (4, 257, 1), (4, 8, 0), (4, 8, 9), (4, 64, 17), ((1 << 29) + 1, 8, 2)):
         refuses(fl, be, lambda: be.routing(rows, experts, k), "Routing")
     r = be.routing(8, 4, 2)
     refuses(fl, be, lambda: r.linear(new(8, 16), new(64, 16)), "nothing routed")
@@ -585,7 +584,10 @@ def test_refusals(fl, be):
     refuses(fl, be, lambda: be.wrap(0, 2, 2, fl.F32), "device memory")
     host = np.zeros(16, np.float32)
     refuses(fl, be, lambda: be.wrap(host.ctypes.data, 2, 2, fl.F32), "device memory")
-    refuses(fl, be, lambda: be.wrap(wide.ptr() + 1, 2, 2, fl.BF16), "aligned")
+    refuses(fl, be, lambda: be.wrap(wide.ptr() + 16, 2, 2, fl.BF16), "aligned")
+    full = be.routing(8, 4, 4)
+    own = be.wrap(full.device_pointers()["weights"], 8, 4, fl.F32)
+    refuses(fl, be, lambda: full.route(own), "overlap")
     refuses(fl, be, lambda: be.wrap(wide.ptr(), -1, 2, fl.BF16), "shape")
     refuses(fl, be, lambda: be.wrap(wide.ptr(), 2, 2, 3), "dtype")
     be.synchronize()
@@ -602,3 +604,16 @@ def test_wrapped_weight_follows_its_memory(fl, be):
     w.fill_(2.0)
     torch.cuda.synchronize()
     assert (x.linear(x, t, None).to_host() == 128).all()
+    y = be.new_tensor(4, 128, None, fl.BF16)
+    call = lambda: be.check(fl.lib().Cuda_Linear_Fused(be.ctx, x.buf, 4, 64, t.buf, 128, None, y.buf, 0))  # noqa: E731
+    g, stream = torch.cuda.CUDAGraph(), torch.cuda.ExternalStream(be.stream())
+    call()
+    be.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        call()
+    w.fill_(3.0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        g.replay()
+    be.synchronize()
+    assert (y.to_host() == 192).all()
