@@ -325,7 +325,6 @@ CudaBufferRef Cuda_WrapTensor(CudaContextRef ctx, void* ptr, int64_t rows, int64
   const int64_t es = dtype_size(dtype);
   if (rows < 0 || cols < 0 || (cols > 0 && rows > INT64_MAX / es / cols)) return refuse("bad shape");
   if (rows * cols > 0) {
-    if ((uintptr_t)ptr % 32 != 0) return refuse("pointer not aligned to 32 bytes");  // the kernels' widest access
     cudaPointerAttributes at{};
     if (!ptr || cudaPointerGetAttributes(&at, ptr) != cudaSuccess ||
         (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)) {
@@ -333,6 +332,7 @@ CudaBufferRef Cuda_WrapTensor(CudaContextRef ctx, void* ptr, int64_t rows, int64
       return refuse("not device memory");
     }
     if (at.type == cudaMemoryTypeDevice && at.device != c->device) return refuse("memory of another device");
+    if ((uintptr_t)ptr % 32 != 0) return refuse("pointer not aligned to 32 bytes");  // the kernels' widest access
   }
   Buf* b = new Buf();
   b->ctx = c;

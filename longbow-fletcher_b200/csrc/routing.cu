@@ -477,15 +477,24 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArg
   pdl_wait();
   const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
   const int64_t p0 = r0 * a.k, p1 = r0 < r1 ? r1 * a.k : p0;
+  // A run's experts are on their way while the block finds its first slots, or ranks the run before.
+  int32_t next[kSub / kThreads];
+  auto fetch = [&](int64_t p) {
+#pragma unroll
+    for (int i = 0; i < kSub / kThreads; i++) {
+      const int64_t at_p = p + i * kThreads + threadIdx.x;
+      next[i] = at_p < p1 ? a.experts[at_p] : -1;
+    }
+  };
+  fetch(p0);
   for (int e = threadIdx.x; e < a.E; e += kThreads) at[e] = a.offsets[e] + a.hist[(int64_t)e * a.stride + blockIdx.x];
   for (int64_t p = p0; p < p1; p += kSub) {
-    const int n = (int)(p1 - p < kSub ? p1 - p : kSub);
     __syncthreads();  // the last run's ids and counts have been read
 #pragma unroll
-    for (int i = 0; i < kSub; i += kThreads)
-      if (i + (int)threadIdx.x < n) ids[i + threadIdx.x] = (int16_t)a.experts[p + i + threadIdx.x];
+    for (int i = 0; i < kSub / kThreads; i++) ids[i * kThreads + threadIdx.x] = (int16_t)next[i];
+    if (p + kSub < p1) fetch(p + kSub);
     __syncthreads();
-    assign_slots(a, p, n, ids, at, count);
+    assign_slots(a, p, (int)(p1 - p < kSub ? p1 - p : kSub), ids, at, count);
   }
 }
 
