@@ -3,9 +3,9 @@
 // A row belongs to L lanes, which read its logits in chunks of eight.  A candidate is one integer key:
 // the logit's bits in an order that compares like the value, above the complement of the expert's
 // index, so the largest key is the largest logit and, among equals, the lowest expert (32 bits for
-// 16-bit logits, else 64).  Each lane keeps its KM >= top_k largest keys in order (a sorting network
-// for the first chunk, an insertion for each later key above the smallest); then a round takes the
-// largest of the lanes' first keys (log2 L shuffles) and its owner moves on.  Lane j mod L keeps
+// 16-bit logits, else 64).  Each lane keeps its KM >= top_k largest keys in order (networks sort a chunk
+// and merge it in; two choices are kept by insertion); then a round takes the largest of the lanes'
+// first keys (log2 L shuffles) and its owner moves on.  Lane j mod L keeps
 // choice j and computes its exponential, with the first winner as the maximum.  Bound by instruction
 // issue: L = 4 lanes a row for many rows (65536 x 64 -> 6: 82 instructions a row, against 164 with 8
 // lanes that hold eight keys each), a whole warp a row where rows are few and latency counts.
@@ -158,6 +158,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
   load(r0 + threadIdx.x / L, gl * V, next);
   for (int64_t base = r0; base < r1; base += kPass) {
     const int64_t mine = base + threadIdx.x / L;
+    if (base + (threadIdx.x & ~31) / L >= r1) break;  // none of the warp's rows is left
     K list[KM] = {};
     float ref = 0.f, sum = 0.f, top = -INFINITY;  // sum of exp(x - ref) over the lane's logits, their maximum
     for (int c = 0; c < chunks; c++) {
@@ -184,11 +185,22 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
         }
         sum += s1;
       }
-      if (KM >= V && c == 0) {
+      if constexpr (KM >= V) {
+        // The chunk in order; the larger of its i-th last and the list's last eight, pairwise, leave the KM
+        // largest in a bitonic sequence, which log2 KM steps put in order.
         sort8(key);
+        if (c == 0) {
 #pragma unroll
-        for (int i = 0; i < V; i++)
-          if (i < KM) list[i] = key[i];
+          for (int i = 0; i < V; i++) list[i] = key[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i++) list[KM - V + i] = key[V - 1 - i] > list[KM - V + i] ? key[V - 1 - i] : list[KM - V + i];
+#pragma unroll
+          for (int d = KM / 2; d >= 1; d /= 2)
+#pragma unroll
+            for (int i = 0; i < KM; i++)
+              if ((i & d) == 0) exchange(list[i], list[i + d]);
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < V; i++) {
@@ -571,7 +583,7 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
     a.chunk = (a.rows + blocks - 1) / blocks;
   } else {
     blocks = std::min<int64_t>(blocks, max_blocks(c));
-    a.chunk = ((a.rows + blocks - 1) / blocks + pass - 1) / pass * pass;  // whole turns
+    a.chunk = (a.rows + blocks - 1) / blocks;
     blocks = (a.rows + a.chunk - 1) / a.chunk;
   }
   const int n = (int)blocks;
