@@ -10,12 +10,12 @@
 // issue: L = 4 lanes a row for many rows (65536 x 64 -> 6: 82 instructions a row, against 164 with 8
 // lanes that hold eight keys each), a whole warp a row where rows are few and latency counts.
 //
-// Grouping is a stable counting sort in two launches: k_route leaves, per block of rows, how many
-// choices each expert got, and its last block to finish turns these into what precedes each block;
-// k_group ranks its pairs within the block and writes slots and their inverse.  (Summed by every
-// block of k_group instead, the same lines of L2 are read by all at once: 9 of 19 us.)  Where a cluster
-// of blocks can hold all pairs, its blocks read one another's counts and one launch does it all.
-// Nothing in the result depends on which block is last, so the slots are the same in every run.
+// Grouping is a stable counting sort in two launches: k_route leaves, per block of rows and per run of
+// kSpan blocks, how many choices each expert got; k_group sums the runs and blocks before its own, ranks
+// its pairs within the block, and writes slots and their inverse.  (With the blocks' counts alone every
+// block reads the same lines of L2 at once: 9 of 19 us; summed by the last block of k_route: 4 us.)
+// Where a cluster of blocks can hold all pairs, its blocks read one another's counts and one launch does
+// it all.  Only integers are added in no fixed order, so the slots are the same in every run.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -28,6 +28,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBlocksPerSM = 2;
 constexpr int V = 8;  // logits per lane
+constexpr int kSpan = 16;
 // Keys of eight logits from expert e0 on, and the logits in fp32.  NaN counts as -inf and -0 as +0;
 // a key that is not `valid` (-inf, or the 0 of an empty place) is never chosen.
 template <typename T>
@@ -110,9 +111,9 @@ struct RouteArgs {
   int32_t* slots;
   int32_t* pair_of;
   int32_t* offsets;
-  int32_t* hist;    // [E, stride]
-  int32_t* ticket;  // blocks of k_route that have finished; 0 between launches
-  int32_t stride;
+  int32_t* hist;    // [blocks, E] choices of each expert in a block's rows
+  int32_t* spans;   // [blocks / kSpan, E] the same for runs of blocks; 0 between calls
+  int32_t* ticket;  // blocks of k_group that have read them; 0 between calls
 };
 
 // e^d on the special-function unit: d's product with log2 e is rounded once, so the relative error is
@@ -422,70 +423,22 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
     if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // nobody reads this block's now
   } else {
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += kThreads) a.hist[(int64_t)e * a.stride + blockIdx.x] = hist[e];
-    __shared__ bool last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = gridDim.x;
-    if (threadIdx.x == 0) *a.ticket = 0;
-    // Counts become exclusive sums over the blocks: a warp an expert, four blocks a lane, the counts of
-    // four experts on their way at once.
-    constexpr int TURNS = 3, AT_ONCE = 4;  // 3 * 128 >= max_blocks
-    const int quads = (blocks + 3) / 4;
-    for (int e0 = warp; e0 < a.E; e0 += AT_ONCE * kWarps) {
-      int4 v[AT_ONCE][TURNS];
-#pragma unroll
-      for (int q = 0; q < AT_ONCE; q++)
-#pragma unroll
-        for (int i = 0; i < TURNS; i++) {
-          const int e = e0 + q * kWarps, at4 = i * 32 + lane;
-          v[q][i] = e < a.E && at4 < quads ? __ldcg(reinterpret_cast<const int4*>(a.hist + (int64_t)e * a.stride) + at4)
-                                           : make_int4(0, 0, 0, 0);
-        }
-#pragma unroll
-      for (int q = 0; q < AT_ONCE; q++) {
-        const int e = e0 + q * kWarps;
-        if (e >= a.E) break;
-        int32_t carry = 0;
-#pragma unroll
-        for (int i = 0; i < TURNS; i++) {
-          const int at4 = i * 32 + lane;
-          int4 n = v[q][i];
-          if (4 * at4 + 1 >= blocks) n.y = 0;  // behind the last block
-          if (4 * at4 + 2 >= blocks) n.z = 0;
-          if (4 * at4 + 3 >= blocks) n.w = 0;
-          const int32_t mine = n.x + n.y + n.z + n.w;
-          int32_t s = mine;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += u;
-          }
-          const int32_t b = carry + s - mine;
-          if (at4 < quads)
-            reinterpret_cast<int4*>(a.hist + (int64_t)e * a.stride)[at4] =
-                make_int4(b, b + n.x, b + n.x + n.y, b + n.x + n.y + n.z);
-          carry += __shfl_sync(0xffffffffu, s, 31);
-        }
-        if (lane == 0) hist[e] = carry;
-      }
+    for (int e = threadIdx.x; e < a.E; e += kThreads) {
+      const int32_t n = hist[e];
+      a.hist[(int64_t)blockIdx.x * a.E + e] = n;
+      if (n) atomicAdd(&a.spans[(int64_t)(blockIdx.x / kSpan) * a.E + e], n);
     }
-    __syncthreads();
-    const int32_t total = scan_experts(hist, at, a.E, tmp);
-    for (int e = threadIdx.x; e < a.E; e += kThreads) a.offsets[e] = at[e];
-    if (threadIdx.x == 0) a.offsets[a.E] = total;
   }
 }
 
 // One block per block of k_route, the same rows.
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArgs a) {
-  __shared__ int32_t at[kMaxExperts];
+  __shared__ int32_t at[kMaxExperts], before[kMaxExperts], all[kMaxExperts], tmp[kWarps + 1];
   __shared__ int16_t ids[kSub];
+  __shared__ bool last;
   extern __shared__ int32_t count[];
+  for (int e = threadIdx.x; e < a.E; e += kThreads) before[e] = all[e] = 0;
+  __syncthreads();
   pdl_wait();
   const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
   const int64_t p0 = r0 * a.k, p1 = r0 < r1 ? r1 * a.k : p0;
@@ -499,7 +452,39 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArg
     }
   };
   fetch(p0);
-  for (int e = threadIdx.x; e < a.E; e += kThreads) at[e] = a.offsets[e] + a.hist[(int64_t)e * a.stride + blockIdx.x];
+  // kThreads / E threads share an expert's counts.
+  const int spans = (gridDim.x + kSpan - 1) / kSpan, mine = blockIdx.x / kSpan;
+  const int share = kThreads / a.E, e = threadIdx.x % a.E, part = threadIdx.x / a.E;
+  if (part < share) {
+    int32_t b = 0, n = 0;
+#pragma unroll 4
+    for (int i = part; i < spans; i += share) {
+      const int32_t v = __ldcg(&a.spans[(int64_t)i * a.E + e]);
+      n += v;
+      b += i < mine ? v : 0;
+    }
+#pragma unroll 4
+    for (int i = mine * kSpan + part; i < (int)blockIdx.x; i += share) b += __ldcg(&a.hist[(int64_t)i * a.E + e]);
+    atomicAdd(&before[e], b);
+    atomicAdd(&all[e], n);
+  }
+  __syncthreads();
+  // The last block to have read the runs' counts clears them for the next call.
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
+  }
+  const int32_t total = scan_experts(all, at, a.E, tmp);
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < a.E; i += kThreads) a.offsets[i] = at[i];
+    if (threadIdx.x == 0) a.offsets[a.E] = total;
+  }
+  if (last) {
+    for (int i = threadIdx.x; i < spans * a.E; i += kThreads) a.spans[i] = 0;
+    if (threadIdx.x == 0) *a.ticket = 0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.E; i += kThreads) at[i] += before[i];
   for (int64_t p = p0; p < p1; p += kSub) {
     __syncthreads();  // the last run's ids and counts have been read
 #pragma unroll
@@ -534,7 +519,11 @@ int32_t route_l(Ctx* c, const RouteArgs& a, int blocks, bool one) {
   }
   FL_CUDA(c, launch_pdl(k_route<T, L, KM, false>, dim3(blocks), dim3(kThreads), 0, c->stream, a));
   FL_LAUNCH(c);
-  FL_CUDA(c, launch_pdl(k_group, dim3(blocks), dim3(kThreads), smem, c->stream, a));
+  const cudaError_t e = launch_pdl(k_group, dim3(blocks), dim3(kThreads), smem, c->stream, a);
+  if (e != cudaSuccess) {  // nobody clears the runs' counts
+    cudaMemsetAsync(a.spans, 0, (size_t)((blocks + kSpan - 1) / kSpan) * a.E * 4, c->stream);
+    FL_CUDA(c, e);
+  }
   FL_LAUNCH(c);
   return FLETCHER_OK;
 }
@@ -557,8 +546,8 @@ int32_t route_t(Ctx* c, const RouteArgs& a, int blocks, bool one) {
                       : route_k<T, 32>(c, a, blocks, one);
 }
 
-// Rows of int4, at most what the last block's lanes hold.
-int max_blocks(const Ctx* c) { return std::min(kBlocksPerSM * c->num_sms / 4 * 4, 3 * 128); }
+int max_blocks(const Ctx* c) { return kBlocksPerSM * c->num_sms; }
+int64_t max_spans(const Ctx* c) { return (max_blocks(c) + kSpan - 1) / kSpan; }
 
 int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   Ctx* c = r->c;
@@ -570,8 +559,8 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   a.pair_of = r->pair_of;
   a.offsets = r->offsets;
   a.hist = r->hist;
+  a.spans = r->spans;
   a.ticket = r->ticket;
-  a.stride = max_blocks(c);
   const int64_t pass = kThreads / lanes_of(a);  // rows a block takes at once
   const int64_t passes = std::max<int64_t>(1, (a.rows + pass - 1) / pass);
   // One launch where a cluster's blocks hold the pairs and take no more than two turns (4096 x 64 -> 6 in
@@ -645,7 +634,7 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
   r->num_experts = num_experts;
   r->top_k = top_k;
   const int64_t pairs = (max_rows * top_k + 3) / 4 * 4;  // keeps every array 16-byte aligned
-  const int64_t ints = 4 * pairs + (num_experts + 1 + 3) / 4 * 4 + (int64_t)max_blocks(c) * num_experts + 4;
+  const int64_t ints = 4 * pairs + (num_experts + 1 + 3) / 4 * 4 + (max_blocks(c) + max_spans(c)) * num_experts + 1;
   r->bytes = ints * 4;
   const int32_t rc = dev_alloc(c, &r->mem, r->bytes);
   if (rc) {
@@ -658,7 +647,8 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
   r->pair_of = r->experts + 3 * pairs;
   r->offsets = r->experts + 4 * pairs;
   r->hist = r->offsets + (num_experts + 1 + 3) / 4 * 4;
-  r->ticket = r->hist + (int64_t)max_blocks(c) * num_experts;  // 0, as dev_alloc fills
+  r->spans = r->hist + (int64_t)max_blocks(c) * num_experts;
+  r->ticket = r->spans + max_spans(c) * num_experts;  // both 0, as dev_alloc fills
   *out = r;
   return FLETCHER_OK;
 }

@@ -21,8 +21,7 @@ struct Routing {
   int32_t* slots = nullptr;    // [pairs] slot of each pair, -1: none
   int32_t* pair_of = nullptr;  // [pairs] pair of each slot; behind the last slot unspecified
   int32_t* offsets = nullptr;  // [num_experts + 1]
-  int32_t* hist = nullptr;     // [num_experts, blocks] choices of each expert in the rows before a block's
-  int32_t* ticket = nullptr;   // blocks that have counted theirs; 0 between calls
+  int32_t *hist = nullptr, *spans = nullptr, *ticket = nullptr;  // of the counting sort (routing.cu)
   // Cuda_Linear_Grouped's copy of token rows in slot order, grown on demand.  Blocks that were outgrown
   // stay until the routing is freed: captured graphs may still use them.
   static constexpr int kMaxBlocks = 48;
