@@ -441,12 +441,11 @@ class BlockNorm:
         self.c = CBlockNorm(post, pre, eps, residual_scale, branch_scale, 0, gate.rows if gate is not None else 0,
                             **{k: t.buf for k, t in self._tensors.items() if t is not None})
         self._p = ctypes.byref(self.c)
+        self._residual_rows = residual.rows if residual is not None else float("inf")
 
     def _ref(self, rows):
-        for name, need in (("residual", rows), ("gate", self.c.gate_rows)):
-            t = self._tensors[name]
-            if t is not None and t.rows < need:
-                raise FletcherError(1, f"BlockNorm: {name} has {t.rows} rows, {need} are needed")
+        if self._residual_rows < rows:
+            raise FletcherError(1, f"BlockNorm: the residual has {self._residual_rows} rows, {rows} are needed")
         return self._p
 
     def _outputs(self, y, rows, out, out_norm, combine=False):
