@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include <algorithm>
+#include <new>
 
 #include "common.cuh"
 
@@ -334,7 +335,8 @@ CudaBufferRef Cuda_WrapTensor(CudaContextRef ctx, void* ptr, int64_t rows, int64
     if (at.type == cudaMemoryTypeDevice && at.device != c->device) return refuse("memory of another device");
     if ((uintptr_t)ptr % 32 != 0) return refuse("pointer not aligned to 32 bytes");  // the kernels' widest access
   }
-  Buf* b = new Buf();
+  Buf* b = new (std::nothrow) Buf();
+  if (!b) return refuse("out of host memory");
   b->ctx = c;
   b->ptr = ptr;
   b->rows = rows;

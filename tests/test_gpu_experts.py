@@ -498,6 +498,85 @@ def test_expert_block_captured(fl, be):
     del sides
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_no_rows(fl, be, dtype):
+    new = lambda r, c: be.new_tensor(r, c, None, fl.DTYPES[dtype])  # noqa: E731
+    r = be.routing(0, 4, 2)
+    r.route(new(0, 4))
+    got = r.read()
+    assert got["experts"].shape == (0, 2) and (got["offsets"] == 0).all()
+    h = r.linear(new(0, 64), new(4 * 64, 128), None, 4)
+    assert h.dims() == (0, 64)
+    u, n = r.combine(r.linear(h, new(4 * 64, 32), grouped_input=True), fl.BlockNorm(pre=1, residual=new(0, 32)))
+    assert u.dims() == n.dims() == (0, 32)
+    assert new(0, 32).block_norm(fl.BlockNorm(pre=2, gate=new(1, 32)))[1].dims() == (0, 32)
+    be.synchronize()
+
+
+def test_past_32_bits(fl, be):
+    """Outputs and slots of more than 2^31 elements: the last rows against torch."""
+    import torch
+    rows, k, K, N, E = 140000, 2, 64, 8192, 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, K, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(E * K, N, generator=g, device="cuda") / 8).bfloat16()
+    y = torch.empty(rows * k, N, device="cuda", dtype=torch.bfloat16)
+    out = torch.empty(rows, N, device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    wrap = lambda t: be.wrap(t.data_ptr(), *t.shape, fl.BF16)  # noqa: E731
+    r = be.routing(rows, E, k)
+    ids = np.stack([np.arange(rows) % 3, (np.arange(rows) + 1) % 3], 1).astype(np.int32)
+    r.assign(ids)
+    r.linear(wrap(x), wrap(w), out=wrap(y))
+    r.combine(wrap(y), out=wrap(out))
+    slots = torch.from_numpy(r.read()["slots"]).cuda().long()
+    pick = torch.tensor([0, 1, 2, rows // 2, rows - 2, rows - 1], device="cuda")
+    e = torch.from_numpy(ids).cuda()[pick].long()
+    want = torch.einsum("rk,rjkn->rjn", x[pick].double(), w.view(E, K, N)[e].double())
+    mag = torch.einsum("rk,rjkn->rjn", x[pick].double().abs(), w.view(E, K, N)[e].double().abs())
+    got = y[slots[pick]].double()
+    assert ((got - want).abs() <= want.abs() * U["bf16"] + (K + 4) * E24 * mag + 1e-30).all()
+    total = got.sum(1)
+    assert ((out[pick].double() - total).abs() <= total.abs() * U["bf16"] + 4 * E24 * got.abs().sum(1) + 1e-30).all()
+    norm = fl.BlockNorm(pre=fl.NORM_RMS, eps=0.0)
+    wrap(y).block_norm(norm, out_norm=wrap(y))  # in place over 2.3e9 elements
+    be.synchronize()
+    rms = (got * got).mean(2, keepdim=True).sqrt()
+    normed = got / rms
+    assert ((y[slots[pick]].double() - normed).abs() <= normed.abs() * (U["bf16"] + (N + 16) * E24)).all()
+
+
+def test_memory_is_kept_and_returned(fl, be):
+    """A routing's workspace grows on first use only, also across smaller calls, and goes with the routing."""
+    before = be.vram_usage()[0]
+    r = be.routing(512, 4, 2)
+    x, w, y = (be.new_tensor(n, m, None, fl.BF16) for n, m in ((512, 256), (4 * 256, 128), (1024, 128)))
+    small = be.new_tensor(100, 256, None, fl.BF16)
+    r.assign(np.tile([0, 3], (512, 1)))
+    r.linear(x, w, out=y)
+    held = be.vram_usage()[0]
+    r.linear(x, w, out=y)
+    r.assign(np.tile([1, 2], (100, 1)))
+    r.linear(small, w, out=y)
+    assert be.vram_usage()[0] == held
+    del r, x, w, y, small
+    assert be.vram_usage()[0] == before
+
+
+def test_growing_workspace_is_refused_in_a_capture(fl, be):
+    import torch
+    r = be.routing(512, 4, 2)
+    x, w, y = (be.new_tensor(n, m, None, fl.BF16) for n, m in ((512, 256), (4 * 256, 128), (1024, 128)))
+    w2, y2 = be.new_tensor(4 * 128, 64, None, fl.BF16), be.new_tensor(1024, 64, None, fl.BF16)
+    r.assign(np.tile([0, 3], (512, 1)))
+    be.synchronize()
+    g, stream = torch.cuda.CUDAGraph(), torch.cuda.ExternalStream(be.stream())
+    with torch.cuda.graph(g, stream=stream):
+        refuses(fl, be, lambda: r.linear(x, w, out=y), "before capturing")
+        r.linear(y, w2, grouped_input=True, out=y2)  # needs none
+    be.synchronize()
+
+
 def test_calls_are_repeatable(fl, be):
     """The same bits from call to call, between other calls of other sizes."""
     rng = np.random.default_rng(8)
