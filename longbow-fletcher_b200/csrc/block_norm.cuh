@@ -189,7 +189,7 @@ __device__ __forceinline__ void norm_row(float (&v)[NV * VEC], int kind, const f
 
 // A row's inputs are asked for one row ahead: the next y (or the first kAhead choices' rows, whose slots
 // are asked for two rows ahead) while this row is normed, the next residual once this one is used.
-constexpr int kAhead = 2;  // of 16-bit slots; one of fp32 slots, whose registers they take
+constexpr int kAhead = 2;  // one of fp32 slots beside 16-bit rows, which take the registers of two
 // Blocks an SM, by the registers that a row's vectors need (two choices' rows and a residual in flight):
 // 65536 x 768 norms take 78 us with 2, 90 with 3, which spills.
 template <int VEC, int NV>

@@ -7,8 +7,8 @@
 // and merge it in; two choices are kept by insertion); then a round takes the largest of the lanes'
 // first keys (log2 L shuffles) and its owner moves on.  Lane j mod L keeps
 // choice j and computes its exponential, with the first winner as the maximum.  Bound by instruction
-// issue: L = 4 lanes a row for many rows (65536 x 64 -> 6: 82 instructions a row, against 164 with 8
-// lanes that hold eight keys each), a whole warp a row where rows are few and latency counts.
+// issue (65536 x 64 -> 6: 96 warp instructions a row) and the two launches' latency: 17 us.  Four lanes
+// a row for many rows (two and eight were within 1 us there, at 16384 x 128 -> 8 slower by 5 and 1).
 //
 // Grouping is a stable counting sort in two launches: k_route leaves, per block of rows and per run of
 // kSpan blocks, how many choices each expert got; k_group sums the runs and blocks before its own, ranks
@@ -535,8 +535,9 @@ int32_t route_k(Ctx* c, const RouteArgs& a, int blocks, bool one) {
   return route_l<T, L, 16>(c, a, blocks, one);
 }
 
-// Lanes a row: one where a chunk holds all experts; a warp for few rows of many.
-int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E <= 4 * V || a.rows > 2 * kThreads / 32 ? 4 : 32; }
+// Lanes a row: one where a chunk holds all experts; a warp for few rows of many experts, where the chain of
+// chunks is what takes time (128 x 256 -> 8: 6.3 us, 10.3 with four; 32 x 64 -> 6: 6.0 against 4.9).
+int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E > 8 * V && a.rows <= 128 ? 32 : 4; }
 
 template <typename T>
 int32_t route_t(Ctx* c, const RouteArgs& a, int blocks, bool one) {

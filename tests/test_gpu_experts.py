@@ -151,7 +151,7 @@ def check(got, want, tol, dtype, what=""):
 # ---------------------------------------------------------------- routing
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,experts,k", [(1, 8, 2), (0, 8, 2), (1, 1, 1), (7, 3, 3), (300, 9, 1), (513, 17, 16),
-                                            (1000, 64, 6), (2049, 33, 5), (4099, 128, 8), (700, 256, 16), (9001, 200, 3)])
+                                            (1000, 64, 6), (2049, 33, 5), (4099, 128, 8), (700, 256, 16), (9001, 200, 3), (1, 256, 16), (40, 200, 5), (128, 65, 2)])
 def test_routing(fl, be, rows, experts, k, dtype):
     rng = np.random.default_rng(rows * 1000 + experts)
     z = quantise(2 * rng.standard_normal((rows, experts)), dtype)
