@@ -333,8 +333,8 @@ typedef struct FletcherBlockNorm {
  * `rows` rows.  cols <= 49152. */
 int32_t Cuda_BlockNorm(CudaContextRef ctx, CudaBufferRef y, int64_t rows, int64_t cols,
                        const FletcherBlockNorm* norm, CudaBufferRef outResidual, CudaBufferRef outNorm);
-/* Joins the experts' outputs (grouped [slots, cols], as Cuda_Linear_Grouped wrote them, in the other
- * buffers' dtype or f32):
+/* Joins the experts' outputs (grouped [rows*top_k, cols], its slots as Cuda_Linear_Grouped wrote them,
+ * in the other buffers' dtype or f32):
  *   y[r] = sum over the row's choices that have a slot, in order, of weight * grouped[slot]
  * in fp32, followed by Cuda_BlockNorm's u and h of y; norm NULL means u = y.  An output may be the
  * same buffer as the residual or as a gate of `rows` rows, not as `grouped`. */

@@ -577,6 +577,42 @@ def test_growing_workspace_is_refused_in_a_capture(fl, be):
     be.synchronize()
 
 
+def test_two_contexts_at_once(fl, be):
+    """Two contexts on one device, each in a thread of its own, give what each gives alone."""
+    import threading
+    results, errors = {}, []
+
+    def work(name, rounds, seed):
+        try:
+            b = fl.Backend(0)
+            rng = np.random.default_rng(seed)
+            rows, E, k, H, I = (300, 8, 2, 128, 192) if seed else (20, 16, 4, 192, 128)
+            t = {n: tensor(fl, b, rng.standard_normal(s) * f, "bf16") for n, s, f in (
+                ("logits", (rows, E), 1.0), ("x", (rows, H), 1.0), ("up", (E * H, 2 * I), 0.1), ("down", (E * I, H), 0.1))}
+            t["norm"] = fl.BlockNorm(pre=fl.NORM_LAYER, eps=1e-5, residual=t["x"])
+            r = b.routing(rows, E, k)
+            bufs = [b.new_tensor(n, m, None, fl.BF16) for n, m in ((rows * k, I), (rows * k, H), (rows, H))]
+            for _ in range(rounds):
+                block(b, fl, r, t, *bufs, 4)
+            results[name] = bufs[2].to_host()
+            b.synchronize()
+            del r, t, bufs
+            b.close()
+        except Exception as e:  # seen by the test's own thread
+            errors.append(e)
+
+    for seed in (0, 1):
+        work(("alone", seed), 1, seed)
+    threads = [threading.Thread(target=work, args=(("both", seed), 200, seed)) for seed in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for seed in (0, 1):
+        assert (results["both", seed] == results["alone", seed]).all()
+
+
 def test_calls_are_repeatable(fl, be):
     """The same bits from call to call, between other calls of other sizes."""
     rng = np.random.default_rng(8)
