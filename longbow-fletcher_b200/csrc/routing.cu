@@ -336,25 +336,39 @@ __device__ __forceinline__ void assign_slots(const RouteArgs& a, int64_t p0, int
   }
 }
 
-// Exclusive prefix of n[0..E) (shared) into at[0..E), and the total; E <= 256 <= kThreads.
-__device__ __forceinline__ int32_t scan_experts(const int32_t* n, int32_t* at, int E, int32_t* tmp /*[17]*/) {
-  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  int32_t v = t < E ? n[t] : 0, s = v;
+// Exclusive prefix of n (shared, kMaxExperts, 0 past E) into at[0..E), and the total into at[E]; by the
+// block, whose first warp holds eight experts a lane.
+__device__ __forceinline__ void scan_experts(const int32_t* n, int32_t* at, int E) {
+  static_assert(kMaxExperts == 256, "eight a lane");
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int4 v[2] = {reinterpret_cast<const int4*>(n)[2 * lane], reinterpret_cast<const int4*>(n)[2 * lane + 1]};
+    const int32_t sum = (v[0].x + v[0].y + v[0].z + v[0].w) + (v[1].x + v[1].y + v[1].z + v[1].w);
+    int32_t s = sum;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += u;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    s -= sum;  // at[E] and what follows are the total, as nothing is counted there
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int4 q = make_int4(s, s + v[i].x, s + v[i].x + v[i].y, s + v[i].x + v[i].y + v[i].z);
+      reinterpret_cast<int4*>(at)[2 * lane + i] = q;
+      s = q.w + v[i].w;
+    }
+    if (lane == 31) at[kMaxExperts] = s;
   }
-  if (lane == 31) tmp[warp] = s;
   __syncthreads();
-  int32_t before = 0, total = 0;
-  for (int w = 0; w < kWarps; w++) {
-    if (w < warp) before += tmp[w];
-    total += tmp[w];
+}
+
+// The prefix's first slots become this block's, past `before` (null: none); the first block leaves the offsets.
+__device__ __forceinline__ void first_slots(const RouteArgs& a, int32_t* at, const int32_t* before) {
+  for (int e = threadIdx.x; e <= a.E; e += kThreads) {
+    const int32_t v = at[e];
+    if (blockIdx.x == 0) a.offsets[e] = v;
+    if (before && e < a.E) at[e] = v + before[e];
   }
-  if (t < E) at[t] = before + s - v;
-  __syncthreads();
-  return total;
 }
 
 __device__ __forceinline__ int32_t load_shared_of(const int32_t* p, uint32_t rank) {
@@ -371,10 +385,10 @@ __device__ __forceinline__ int32_t load_shared_of(const int32_t* p, uint32_t ran
 constexpr int kClusterMost = 8;
 template <typename T, int L, int KM, bool ONE>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArgs a) {
-  __shared__ int32_t hist[kMaxExperts], at[kMaxExperts], tmp[kWarps + 1];
+  __shared__ __align__(16) int32_t hist[kMaxExperts], at[kMaxExperts + 1];
   extern __shared__ int32_t dyn[];  // ONE: count [kWarps][E], ids [kSub]
   int16_t* ids = ONE ? reinterpret_cast<int16_t*>(dyn + kWarps * a.E) : nullptr;
-  for (int e = threadIdx.x; e < a.E; e += kThreads) hist[e] = 0;
+  for (int e = threadIdx.x; e < kMaxExperts; e += kThreads) hist[e] = 0;
   __syncthreads();
   pdl_wait();
   const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
@@ -390,33 +404,27 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
     }
   }
   if constexpr (ONE) {
-    __shared__ int32_t all[kMaxExperts], before[kMaxExperts];
+    __shared__ __align__(16) int32_t all[kMaxExperts], before[kMaxExperts];
     const bool cluster = gridDim.x > 1;  // the grid is the cluster
-    __syncwarp();
-    if (cluster)
+    if (cluster) {
+      __syncwarp();
       asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    else
-      __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += kThreads) {
-      int32_t n = 0, b = 0;
-      for (uint32_t r = 0; r < gridDim.x; r++) {
-        const int32_t v = cluster ? load_shared_of(&hist[e], r) : hist[e];
-        n += v;
-        if (r < blockIdx.x) b += v;
+      for (int e = threadIdx.x; e < kMaxExperts; e += kThreads) {
+        int32_t n = 0, b = 0;
+        for (uint32_t r = 0; e < a.E && r < gridDim.x; r++) {
+          const int32_t v = load_shared_of(&hist[e], r);
+          n += v;
+          if (r < blockIdx.x) b += v;
+        }
+        all[e] = n;
+        before[e] = b;
       }
-      all[e] = n;
-      before[e] = b;
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' counts are read
     }
-    __syncwarp();
-    if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // the others' counts are read
     __syncthreads();
-    const int32_t total = scan_experts(all, at, a.E, tmp);
-    if (blockIdx.x == 0) {
-      for (int e = threadIdx.x; e < a.E; e += kThreads) a.offsets[e] = at[e];
-      if (threadIdx.x == 0) a.offsets[a.E] = total;
-      __syncthreads();
-    }
-    for (int e = threadIdx.x; e < a.E; e += kThreads) at[e] += before[e];
+    scan_experts(cluster ? all : hist, at, a.E);
+    first_slots(a, at, cluster ? before : nullptr);
     __syncthreads();
     if (r0 < r1) assign_slots(a, r0 * a.k, (int)((r1 - r0) * a.k), ids, at, dyn);
     __syncwarp();
@@ -433,11 +441,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_route(const RouteArg
 
 // One block per block of k_route, the same rows.
 __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArgs a) {
-  __shared__ int32_t at[kMaxExperts], before[kMaxExperts], all[kMaxExperts], tmp[kWarps + 1];
+  __shared__ __align__(16) int32_t at[kMaxExperts + 1], before[kMaxExperts], all[kMaxExperts];
   __shared__ int16_t ids[kSub];
   __shared__ bool last;
   extern __shared__ int32_t count[];
-  for (int e = threadIdx.x; e < a.E; e += kThreads) before[e] = all[e] = 0;
+  for (int e = threadIdx.x; e < kMaxExperts; e += kThreads) before[e] = all[e] = 0;
   __syncthreads();
   pdl_wait();
   const int64_t r0 = (int64_t)blockIdx.x * a.chunk, r1 = r0 + a.chunk < a.rows ? r0 + a.chunk : a.rows;
@@ -474,19 +482,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArg
     __threadfence();
     last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
   }
-  const int32_t total = scan_experts(all, at, a.E, tmp);
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < a.E; i += kThreads) a.offsets[i] = at[i];
-    if (threadIdx.x == 0) a.offsets[a.E] = total;
-  }
+  scan_experts(all, at, a.E);
+  first_slots(a, at, before);
   if (last) {
     for (int i = threadIdx.x; i < spans * a.E; i += kThreads) a.spans[i] = 0;
     if (threadIdx.x == 0) *a.ticket = 0;
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.E; i += kThreads) at[i] += before[i];
   for (int64_t p = p0; p < p1; p += kSub) {
-    __syncthreads();  // the last run's ids and counts have been read
+    __syncthreads();  // the first slots stand; the last run's ids and counts have been read
 #pragma unroll
     for (int i = 0; i < kSub / kThreads; i++) ids[i * kThreads + threadIdx.x] = (int16_t)next[i];
     if (p + kSub < p1) fetch(p + kSub);
