@@ -539,7 +539,7 @@ int32_t route_k(Ctx* c, const RouteArgs& a, int blocks, bool one) {
 }
 
 // Lanes a row: one where a chunk holds all experts; a warp for few rows of many experts, where the chain of
-// chunks is what takes time (128 x 256 -> 8: 6.3 us, 10.3 with four; 32 x 64 -> 6: 6.0 against 4.9).
+// chunks is what takes time (128 x 256 -> 8: 6.1 us, 9.6 with four; 32 x 64 -> 6: 5.3 against 4.2).
 int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E > 8 * V && a.rows <= 128 ? 32 : 4; }
 
 template <typename T>
@@ -568,7 +568,7 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   const int64_t pass = kThreads / lanes_of(a);  // rows a block takes at once
   const int64_t passes = std::max<int64_t>(1, (a.rows + pass - 1) / pass);
   // One launch where a cluster's blocks hold the pairs and take no more than two turns (4096 x 64 -> 6 in
-  // four turns: 16.8 us, in two launches 10.7; 4096 x 8 -> 2: 5.7 against 9.0).
+  // four turns: 15.9 us, in two launches 9.5; 4096 x 8 -> 2: 5.5 against 7.8).
   const int64_t fit = (a.rows + kSub / a.k - 1) / (kSub / a.k);  // blocks of at most kSub pairs
   const bool one = fit <= kClusterMost && passes <= 2 * kClusterMost;
   int64_t blocks = std::max(fit, std::min<int64_t>(passes, one ? kClusterMost : max_blocks(c)));
