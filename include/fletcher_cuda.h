@@ -268,7 +268,11 @@ int32_t Cuda_MeanPoolL2(CudaContextRef ctx, CudaBufferRef hidden, const int32_t*
  * 1 <= top_k <= min(16, num_experts), max_rows * top_k <= 2^30.
  * A routing's device memory belongs to its context (as a buffer's does): free it before the
  * context.  The next Cuda_Routing_TopK or Assign overwrites it in stream order; graphs that share
- * one routing must not run at the same time. */
+ * one routing must not run at the same time.
+ * Calls take their number of rows from the last Cuda_Routing_TopK or Assign that was called, captured
+ * ones included.  Where the device holds another routing by then (a replayed graph's, or an earlier
+ * one while the last is only captured), they stay within those rows: what lies past them is neither
+ * read nor written, and outputs mean something again after the next routing. */
 int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_experts, int32_t top_k,
                             CudaRoutingRef* out);
 int32_t Cuda_Routing_Free(CudaRoutingRef routing);

@@ -139,6 +139,7 @@ int32_t Cuda_Combine_Grouped(CudaRoutingRef routing, CudaBufferRef grouped, int6
   a.slots = r->slots;
   a.weights = r->weights;
   a.top_k = r->top_k;
+  a.num_slots = (int32_t)r->pairs();
   return launch_combine(c, u ? u->dtype : h->dtype, yb->dtype, a);
 }
 

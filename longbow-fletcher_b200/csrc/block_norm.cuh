@@ -26,6 +26,7 @@ struct NormArgs {
   const int32_t* slots;  // combine: [rows, top_k]
   const float* weights;
   int32_t top_k;
+  int32_t num_slots;     // slots from here on are none (GroupedArgs)
   const void* residual;  // null: 0
   const void* gate;      // null: 1
   int64_t gate_step;     // elements from one row's gate to the next: 0 or cols
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
     s = -1;
     if (r < a.rows && lane < a.top_k) {
       s = a.slots[r * a.top_k + lane];
+      if (s >= a.num_slots) s = -1;
       f = a.weights[r * a.top_k + lane];
     }
   };
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs 
       if constexpr (COMBINE) {
         for (int j = 0; j < a.top_k; j++) {
           const int32_t slot = a.slots[row * a.top_k + j];
-          if (slot >= 0) s = fmaf(a.weights[row * a.top_k + j], to_f<TY>(y[(int64_t)slot * a.cols + c]), s);
+          if (slot >= 0 && slot < a.num_slots) s = fmaf(a.weights[row * a.top_k + j], to_f<TY>(y[(int64_t)slot * a.cols + c]), s);
         }
       } else {
         s = to_f<TY>(y[row * a.cols + c]);

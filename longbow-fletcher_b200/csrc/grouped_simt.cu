@@ -8,14 +8,15 @@ namespace fl {
 namespace {
 
 // The block's group and rows: m-tile `tile` of all groups' m-tiles in order; the tile's first slot
-// and the group's end, expert -1 when there are fewer tiles.  Called by one warp.
-__device__ __forceinline__ void find_tile(const int32_t* __restrict__ offsets, int E, int tile, int rows_per_tile,
-                                          int32_t* expert, int32_t* first, int32_t* end) {
+// and the group's end, expert -1 when there are fewer tiles.  No slot lies past `pairs` (GroupedArgs).
+// Called by one warp.
+__device__ __forceinline__ void find_tile(const int32_t* __restrict__ offsets, int E, int32_t pairs, int tile,
+                                          int rows_per_tile, int32_t* expert, int32_t* first, int32_t* end) {
   const int lane = threadIdx.x & 31;
   int before = 0, e_found = -1, f = 0, n = 0;
   for (int b = 0; b < E; b += 32) {
     const int e = b + lane;
-    const int32_t o0 = e < E ? offsets[e] : 0, o1 = e < E ? offsets[e + 1] : 0;
+    const int32_t o0 = e < E ? min(offsets[e], pairs) : 0, o1 = e < E ? min(offsets[e + 1], pairs) : 0;
     const int tiles = (o1 - o0 + rows_per_tile - 1) / rows_per_tile;
     int s = tiles;
 #pragma unroll
@@ -74,7 +75,8 @@ __global__ void __launch_bounds__((BM / TM) * (BN / TN) * KS) k_grouped_simt(con
   };
   const unsigned nt = (unsigned)((a.n_out + BN - 1) / BN);  // n-tiles, fastest
   pdl_wait();
-  if (threadIdx.x < 32) find_tile(a.offsets, a.experts, (int)(blockIdx.x / nt), BM, &s_tile[0], &s_tile[1], &s_tile[2]);
+  if (threadIdx.x < 32)
+    find_tile(a.offsets, a.experts, (int32_t)a.pairs, (int)(blockIdx.x / nt), BM, &s_tile[0], &s_tile[1], &s_tile[2]);
   __syncthreads();
   const int e = s_tile[0];
   if (e < 0) return;
@@ -86,7 +88,7 @@ __global__ void __launch_bounds__((BM / TM) * (BN / TN) * KS) k_grouped_simt(con
 #pragma unroll
   for (int i = 0; i < XL; i++) {
     const int s = first + xm + i * (kThreads / BK);
-    const int64_t r = s >= end ? -1 : a.pair_of ? a.pair_of[s] / a.top_k : s;
+    const int64_t r = s >= end ? -1 : a.pair_of ? min((int64_t)(a.pair_of[s] / a.top_k), a.x_rows - 1) : s;
     xrow[i] = r < 0 ? nullptr : reinterpret_cast<const T*>(a.x) + r * a.K + xk;
   }
   const T* w = reinterpret_cast<const T*>(a.w) + (int64_t)e * a.K * a.N + n0 + wn;

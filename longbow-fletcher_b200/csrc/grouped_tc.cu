@@ -75,6 +75,7 @@ struct Args {
   int64_t N, n_out;
   int32_t E, top_k, num_kb, n_tiles, act;
   int32_t out32;  // fp32 result
+  int32_t pairs, last_row;  // bounds of the slots and of x's rows (GroupedArgs)
 };
 
 template <bool PAIR>
@@ -105,14 +106,15 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
   return d;
 }
 
-// Copies the offsets to shared memory and counts the groups' row tiles; by the whole block.
-__device__ __forceinline__ int fill_table(const int32_t* offsets, int E, int tile_m, int32_t* offs, int32_t* tmp) {
+// Copies the offsets to shared memory, none past `pairs`, and counts the groups' row tiles; by the whole block.
+__device__ __forceinline__ int fill_table(const int32_t* offsets, int E, int32_t pairs, int tile_m, int32_t* offs,
+                                          int32_t* tmp) {
   const int t = threadIdx.x, warp = t >> 5, warps = blockDim.x >> 5;
   int n = 0;
   for (int e = t; e <= E; e += blockDim.x) {
-    const int o = offsets[e];
+    const int o = min(offsets[e], pairs);
     offs[e] = o;
-    if (e < E) n += (offsets[e + 1] - o + tile_m - 1) / tile_m;
+    if (e < E) n += (min(offsets[e + 1], pairs) - o + tile_m - 1) / tile_m;
   }
   n = __reduce_add_sync(0xffffffffu, n);
   if ((t & 31) == 0) tmp[warp] = n;
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   pdl_wait();  // the routing and x are the previous kernels' work
-  const int num_tiles = fill_table(args.offsets, args.E, C::TILE_M, offs, tmp) * args.n_tiles;
+  const int num_tiles = fill_table(args.offsets, args.E, args.pairs, C::TILE_M, offs, tmp) * args.n_tiles;
   tc_fence_before();
   if constexpr (PAIR)
     cluster_sync();  // both CTAs' barriers are initialised before any cross-CTA signal
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();  // the routing and x are the previous kernels' work
-  const int num_tiles = fill_table(args.offsets, args.E, C::TILE_M, offs, tmp) * args.n_tiles;
+  const int num_tiles = fill_table(args.offsets, args.E, args.pairs, C::TILE_M, offs, tmp) * args.n_tiles;
   // SPLIT: this CTA's tile (its cluster's) and range of K slabs; else all tiles with a stride, all slabs.
   const int ranks = SPLIT ? (int)cluster_ctas() : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
   const int first_tile = SPLIT ? (int)blockIdx.x / ranks : (int)blockIdx.x;
@@ -558,7 +560,8 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const int s = t.first + 4 * lane + i;
-          rows[i] = args.pair_of[s < t.end ? s : t.first] / args.top_k;  // past the group: computed, not stored
+          // past the group: computed, not stored
+          rows[i] = min(args.pair_of[s < t.end ? s : t.first] / args.top_k, args.last_row);
         }
       }
       for (int kb = kb0; kb < kb1; kb++) {
@@ -731,6 +734,8 @@ Args args_of(const Ctx* c, const GroupedArgs& g, int out_n) {
   a.n_tiles = (int)((g.n_out + out_n - 1) / out_n);
   a.act = g.act;
   a.out32 = g.out32;
+  a.pairs = (int32_t)g.pairs;
+  a.last_row = (int32_t)g.x_rows - 1;
   return a;
 }
 
@@ -842,13 +847,14 @@ int32_t pick(Ctx* c, int32_t dt, const GroupedArgs& g) {
 // Token rows copied to their slots: a warp a token, whose row is read once and written for each of its
 // choices.  Bound by HBM at (1 + top_k) * rows * K * 2 bytes.
 __global__ void __launch_bounds__(256) k_place_rows(const uint4* __restrict__ x, const int32_t* __restrict__ slots,
-                                                    int64_t rows, int top_k, int vecs, uint4* __restrict__ out) {
+                                                    int64_t rows, int top_k, int vecs, int pairs,
+                                                    uint4* __restrict__ out) {
   pdl_wait();
   const int lane = threadIdx.x & 31;
   for (int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < rows;
        t += ((int64_t)gridDim.x * blockDim.x) >> 5) {
     const uint4* src = x + t * vecs;
-    const int mine = lane < top_k ? slots[t * top_k + lane] : -1;
+    const int slot_of = lane < top_k ? slots[t * top_k + lane] : -1, mine = slot_of < pairs ? slot_of : -1;
     for (int v0 = 0; v0 < vecs; v0 += 128) {
       uint4 q[4];
 #pragma unroll
@@ -907,7 +913,7 @@ int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& args, void* 
   if (g.slots && !gathers(g)) {
     const int64_t blocks = std::min<int64_t>((g.x_rows + 7) / 8, (int64_t)c->num_sms * 8);
     FL_CUDA(c, launch_pdl(tcg::k_place_rows, dim3((unsigned)blocks), dim3(256), 0, c->stream, (const uint4*)g.x, g.slots,
-                          g.x_rows, g.top_k, (int)(g.K / 8), (uint4*)workspace));
+                          g.x_rows, g.top_k, (int)(g.K / 8), (int)g.pairs, (uint4*)workspace));
     FL_LAUNCH(c);
     g.x = workspace;
     g.x_rows = g.pairs;

@@ -47,7 +47,10 @@ inline bool holds(const Ctx* c, const Buf* b, int64_t elems) {
   return b && b->device == c->device && elems >= 0 && elems <= b->bytes / dtype_size(b->dtype);
 }
 
-// What a grouped product reads and writes (grouped_simt.cu, grouped_tc.cu).
+// What a grouped product reads and writes (grouped_simt.cu, grouped_tc.cu).  Buffers are checked against the
+// rows of the last call that routed, but the arrays on the device may be those of another one: a replayed
+// graph's, or an earlier one's while a later one is only captured.  So kernels bound what they read there
+// by `pairs` and `x_rows`, and Cuda_Combine_Grouped's by its slots.
 struct GroupedArgs {
   const void* x;     // [tokens or slots, K]
   const void* w;     // [experts * K, N]
