@@ -253,7 +253,8 @@ int32_t Cuda_MeanPoolL2(CudaContextRef ctx, CudaBufferRef hidden, const int32_t*
  * block follow.  (The reference has the dense block only.)  Shared rules:
  *   - all calls enqueue on the context's stream, read sizes that depend on the routing on the
  *     device alone and never wait for the GPU, so that a sequence of them can be captured into a
- *     CUDA graph (except Cuda_Routing_Assign, which reads host arrays);
+ *     CUDA graph (except Cuda_Routing_Create, Assign and Read, which allocate or use host arrays: during a
+ *     capture they fail and leave it as it was);
  *   - Cuda_Linear_Grouped of token rows keeps a workspace with its routing (up to rows * top_k *
  *     inCols elements, at most doubled), which a call that needs more makes larger; earlier ones
  *     stay valid until the routing is freed.  During a capture it cannot grow: the call fails, so

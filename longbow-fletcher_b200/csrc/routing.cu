@@ -585,6 +585,14 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   return route_t<float>(c, a, n, one);
 }
 
+// For calls that allocate, read host arrays or wait: a graph cannot hold them.
+int32_t refuse_capture(Ctx* c, const char* what) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  FL_CUDA(c, cudaStreamIsCapturing(c->stream, &st));
+  FL_CHECK(c, st == cudaStreamCaptureStatusNone, "Routing: %s cannot be captured", what);
+  return FLETCHER_OK;
+}
+
 }  // namespace
 
 int32_t routing_workspace(Routing* r, int64_t bytes, void** out) {
@@ -630,6 +638,8 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
            std::min(kMaxTopK, num_experts));
   FL_CHECK(c, max_rows >= 0 && max_rows <= ((int64_t)1 << 30) / top_k, "Routing: %lld rows are too many",
            (long long)max_rows);
+  int32_t rc = refuse_capture(c, "Create");
+  if (rc) return rc;
   Routing* r = new (std::nothrow) Routing();
   if (!r) return set_error(c, FLETCHER_ERR_OOM, "Routing: out of host memory");
   r->c = c;
@@ -640,8 +650,7 @@ int32_t Cuda_Routing_Create(CudaContextRef ctx, int64_t max_rows, int32_t num_ex
   const int64_t pairs = (max_rows * top_k + 3) / 4 * 4;  // keeps every array 16-byte aligned
   const int64_t ints = 4 * pairs + (num_experts + 1 + 3) / 4 * 4 + (max_blocks(c) + max_spans(c)) * num_experts + 1;
   r->bytes = ints * 4;
-  const int32_t rc = dev_alloc(c, &r->mem, r->bytes);
-  if (rc) {
+  if ((rc = dev_alloc(c, &r->mem, r->bytes))) {
     delete r;
     return rc;
   }
@@ -709,9 +718,10 @@ int32_t Cuda_Routing_Assign(CudaRoutingRef routing, const int32_t* experts, cons
   for (int64_t i = 0; i < pairs; i++)
     FL_CHECK(c, experts[i] >= -1 && experts[i] < r->num_experts, "Routing: expert %d outside [-1, %d)", experts[i],
              r->num_experts);
-  r->rows = -1;
-  int32_t rc = stage_to_device(c, r->experts, experts, pairs * 4);
+  int32_t rc = refuse_capture(c, "Assign");
   if (rc) return rc;
+  r->rows = -1;
+  if ((rc = stage_to_device(c, r->experts, experts, pairs * 4))) return rc;
   if (weights) {
     rc = stage_to_device(c, r->weights, weights, pairs * 4);
   } else {
@@ -738,6 +748,8 @@ int32_t Cuda_Routing_Read(CudaRoutingRef routing, int32_t* experts, float* weigh
   DeviceGuard g(c);
   FL_CHECK(c, r->device == c->device, "Routing: made on another device");
   FL_CHECK(c, r->rows >= 0, "Routing: nothing routed yet");
+  const int32_t rc = refuse_capture(c, "Read");
+  if (rc) return rc;
   const size_t n = (size_t)r->pairs() * 4;
   const struct {
     void* to;

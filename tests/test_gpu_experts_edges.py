@@ -59,3 +59,25 @@ def test_rows_of_another_routing_stay_out(fl, be, rows, N, K, dtype):  # noqa: F
     assert (np.abs(got[:rows * k] - want) <= np.abs(want) * U[dtype] * 1.01 + (K + 4) * E24 * 64).all()
     assert np.isnan(got[rows * k:]).all()
     del g
+
+
+def test_what_cannot_be_captured_is_refused(fl, be):  # noqa: F811
+    """Create, Assign and Read fail during a capture, which goes on, and so does the routing."""
+    r = be.routing(4, 4, 2)
+    z = np.array([[0, 1, 2, 3], [3, 2, 1, 0]], np.float32)
+    t = tensor(fl, be, z, "f32")
+    r.assign(np.array([[1, 0], [2, 3], [0, 1]]))
+
+    def calls():
+        refuses(fl, be, lambda: be.routing(4, 4, 2), "captured")
+        refuses(fl, be, lambda: r.assign(np.array([[1, 0]])), "captured")
+        refuses(fl, be, lambda: r.read(), "captured")
+        r.route(t)
+
+    g = graph_of(be, calls)
+    for _ in range(2):
+        r.assign(np.array([[0, 1], [2, 3]]))
+        assert (r.read()["experts"] == [[0, 1], [2, 3]]).all()
+        replay(be, g)
+        assert (r.read()["experts"] == [[3, 2], [0, 1]]).all()
+    del g
