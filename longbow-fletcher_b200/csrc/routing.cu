@@ -6,8 +6,10 @@
 // 16-bit logits, else 64).  Each lane keeps its KM >= top_k largest keys in order (networks sort a chunk
 // and merge it in; two choices are kept by insertion); then a round takes the largest of the lanes'
 // first keys (log2 L shuffles) and its owner moves on.  Lane j mod L keeps
-// choice j and computes its exponential, with the first winner as the maximum.  Bound by instruction
-// issue (65536 x 64 -> 6: 96 warp instructions a row) and the two launches' latency: 17 us.  Four lanes
+// choice j and computes its exponential, with the first winner as the maximum; exponentials and quotients
+// are those of full fp32 precision (the special-function unit's took 17.4 us where these take 18.5 and lost
+// up to 16 places where x - m is -30).  Bound by instruction issue for half of its time, else by latency of
+// loads and of the two launches: 65536 x 64 -> 6 in 18.5 us, 16.8 where only chosen weights are summed.  Four lanes
 // a row for many rows (two and eight were within 1 us there, at 16384 x 128 -> 8 slower by 5 and 1).
 //
 // Grouping is a stable counting sort in two launches: k_route leaves, per block of rows and per run of
@@ -116,15 +118,8 @@ struct RouteArgs {
   int32_t* ticket;  // blocks of k_group that have read them; 0 between calls
 };
 
-// e^d on the special-function unit: d's product with log2 e is rounded once, so the relative error is
-// about (|d| + 2) * 2^-24; terms far below the maximum, where that grows, are small.
-__device__ __forceinline__ float exp_fast2(float d) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.44269504f));
-  return y;
-}
 // exp(x - m) where x may equal an infinite m.
-__device__ __forceinline__ float exp_below(float x, float m) { return x == m ? 1.0f : exp_fast2(x - m); }
+__device__ __forceinline__ float exp_below(float x, float m) { return x == m ? 1.0f : expf(x - m); }
 
 // The choices and weights of rows [r0, r1), into `hist` (shared) each expert's count, and, unless null,
 // the choices into `ids` (shared).
@@ -176,13 +171,13 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
 #pragma unroll
         for (int i = 0; i < V; i++) top = fmaxf(top, x[i]);
         const float r = fabsf(top) == INFINITY ? 0.f : top;  // +inf is counted below instead
-        sum = sum > 0.f ? sum * exp_fast2(ref - r) : 0.f;
+        sum = sum > 0.f ? sum * expf(ref - r) : 0.f;
         ref = r;
         float s1 = 0.f;
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
           add2(x[i], x[i + 1], -r, -r);
-          add2(sum, s1, exp_fast2(x[i]), exp_fast2(x[i + 1]));
+          add2(sum, s1, expf(x[i]), expf(x[i + 1]));
         }
         sum += s1;
       }
@@ -249,7 +244,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
       total += w[j];
     }
     if (all) {
-      total = sum > 0.f ? sum * exp_fast2(ref - m) : 0.f;
+      total = sum > 0.f ? sum * expf(ref - m) : 0.f;
       if (m == INFINITY) {  // the row's +inf share the weight
         total = 0.f;
         for (int e = gl; e < a.E; e += L)
@@ -259,7 +254,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     // Divided by the sum first, so that no product overflows before it; 0 where the sum is 0.
-    const float inv = a.sigmoid && !a.normalise ? 1.0f : total > 0.f ? __frcp_rn(total) : 0.f;
+    const float by = a.sigmoid && !a.normalise ? 1.0f : total > 0.f ? total : INFINITY;
     if (mine < r1) {
       const int64_t out = mine * a.k;
 #pragma unroll
@@ -268,7 +263,7 @@ __device__ __forceinline__ void choose(const RouteArgs& a, int64_t r0, int64_t r
         if (j < a.k) {
           const int id = Key::valid(kept[i]) ? Key::expert(kept[i]) : -1;
           a.experts[out + j] = id;
-          a.weights[out + j] = w[i] * inv * a.scale;
+          a.weights[out + j] = w[i] / by * a.scale;
           if (ids) ids[(int)(out - r0 * a.k) + j] = (int16_t)id;
           if (id >= 0) atomicAdd(&hist[id], 1);
         }

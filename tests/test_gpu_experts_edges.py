@@ -81,3 +81,26 @@ def test_what_cannot_be_captured_is_refused(fl, be):  # noqa: F811
         replay(be, g)
         assert (r.read()["experts"] == [[3, 2], [0, 1]]).all()
     del g
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,experts,k", [(3000, 8, 2), (3000, 8, 8), (5000, 40, 2), (100, 96, 8), (4000, 64, 12)])
+def test_routing_weights_are_fp32(fl, be, rows, experts, k, dtype):  # noqa: F811
+    """Weights far below the row's largest are as good as it.  Logits are multiples of 1/4, so that their
+    differences are exact and an exponential is off by expf's own error alone: one place, 2 u."""
+    rng = np.random.default_rng(experts)
+    z = np.round(rng.uniform(-16, 16, (rows, experts)) * 4) / 4  # exact in each type: at most 7 significant bits
+    t = tensor(fl, be, z, dtype)
+    r = be.routing(rows, experts, k)
+    for score, normalise in (("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)):
+        r.route(t, ["softmax", "sigmoid"].index(score), normalise, 2.0)
+        _, want = route_ref(np.float64(z), k, score, normalise, 2.0)
+        one = 2 if score == "softmax" else 4  # exponential; sigmoid also an addition and a division
+        if normalise:  # the chosen are added up and divided by
+            u = one + (one + k - 1) + 1
+        elif score == "softmax":  # so are all, and each chunk of a lane's may scale the sum so far (3: factor, product)
+            u = one + (one + experts - 1 + 3 * (experts // 8 + 1)) + 1
+        else:
+            u = one
+        off = np.abs(r.read()["weights"] - want) / want
+        assert off.max() <= u * E24 * (1 + 1e-5), (score, normalise, off.max() / E24, u)
