@@ -104,3 +104,100 @@ def test_routing_weights_are_fp32(fl, be, rows, experts, k, dtype):  # noqa: F81
             u = one
         off = np.abs(r.read()["weights"] - want) / want
         assert off.max() <= u * E24 * (1 + 1e-5), (score, normalise, off.max() / E24, u)
+
+
+# Shapes of the 256-column products: pairs of SMs gated (2 x 776) and not (1552), single SMs gated (2 x 520) and not (1040).
+WIDE = [(2100, 3, 1, 64, 1552), (1000, 32, 2, 72, 1040)]
+
+
+@pytest.mark.parametrize("rows,experts,k,K,N", WIDE)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("act", [0, 1, 4])
+@pytest.mark.parametrize("bias", [True, False])
+def test_widest_products(fl, be, rows, experts, k, K, N, act, dtype, bias):  # noqa: F811
+    for grouped_input in (False, True):
+        for out in (dtype, "f32"):
+            run_grouped(fl, be, rows, experts, k, K, N, act, dtype, bias, grouped_input, out=out)
+
+
+@pytest.mark.parametrize("rows,experts,k,dtype", [(3000, 40, 12, "bf16"), (2500, 64, 16, "f32"), (5000, 17, 2, "bf16"), (9001, 8, 2, "f16"),
+                                                  (20000, 8, 8, "f32"), (2100, 256, 16, "f16")])
+def test_routing_in_two_launches(fl, be, rows, experts, k, dtype):  # noqa: F811
+    """Every count of choices kept and of lanes a row, where one cluster cannot hold the pairs."""
+    rng = np.random.default_rng(rows)
+    z = quantise(np.round(8 * rng.standard_normal((rows, experts))) / 4, dtype)
+    r = be.routing(rows, experts, k)
+    for _ in range(2):  # the counts are cleared for the next call
+        r.route(tensor(fl, be, z, dtype))
+        got = r.read()
+        ids, w = route_ref(z, k)
+        slots, offsets, _ = group_ref(ids, experts)
+        assert (got["experts"] == ids).all() and (got["slots"] == slots).all() and (got["offsets"] == offsets).all()
+        assert np.allclose(got["weights"], w, rtol=64 * E24, atol=0)
+
+
+def test_graph_outlives_a_growing_workspace(fl, be):  # noqa: F811
+    """A captured product of token rows replays right after a larger one has outgrown its workspace."""
+    rng = np.random.default_rng(5)
+    E, k, K, N = 4, 2, 128, 64
+    small, large = 100, 3000
+    r = be.routing(large, E, k)
+    w = quantise(rng.standard_normal((E * K, N)) / 8, "bf16")
+    tw, z = tensor(fl, be, w, "bf16"), tensor(fl, be, rng.standard_normal((small, E)), "f32")
+    tx, ty = be.new_tensor(small, K, None, fl.BF16), be.new_tensor(small * k, N, None, fl.BF16)
+
+    def calls():
+        r.route(z)
+        r.linear(tx, tw, out=ty)
+
+    calls()
+    g = graph_of(be, calls)
+    held = be.vram_usage()[0]
+    big, out = tensor(fl, be, rng.standard_normal((large, K)), "bf16"), be.new_tensor(large * k, N, None, fl.BF16)
+    r.route(tensor(fl, be, rng.standard_normal((large, E)), "f32"))
+    r.linear(big, tw, out=out)
+    assert be.vram_usage()[0] >= held + large * k * K * 2 + (large * K + large * k * N) * 2
+    for step in range(2):
+        x = quantise(rng.standard_normal((small, K)), "bf16")
+        tx.copy_from_float32(x)
+        big.copy_from_float32(np.zeros((large, K)))
+        replay(be, g)
+        got = ty.to_host()
+        calls()
+        assert (ty.to_host() == got).all()
+        ids = r.read()["experts"]
+        want, tol, _ = grouped_ref(x, w, None, ids, E, 0, False)
+        assert (np.abs(got - want) <= np.abs(want) * U["bf16"] * (1 + 1e-6) + tol * 1.01 + 1e-37).all()
+    del g
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,experts,K,N,act", [(6, 3, 72, 136, 0), (40, 3, 72, 136, 4), (400, 3, 72, 136, 0), (2100, 3, 72, 1552, 0),
+                                                  (2100, 3, 72, 1552, 4), (2000, 32, 72, 1040, 0), (2000, 32, 72, 1040, 4)])
+@pytest.mark.parametrize("grouped_input", [False, True])
+def test_nonfinite_row_stays_alone(fl, be, rows, experts, K, N, act, dtype, grouped_input):  # noqa: F811
+    """A NaN row and an inf row, among finite weights, reach their own slots alone, and an expert's inf and NaN
+    weights that expert's slots alone."""
+    rng = np.random.default_rng(rows)
+    ids = (np.arange(rows) % experts).astype(np.int32)[:, None]
+    order = group_ref(ids, experts)[2]
+    x = quantise(rng.standard_normal((rows, K)), dtype)
+    x[0, :] = np.nan  # of expert 0
+    x[experts + 2, 3] = np.inf  # of expert 2
+    w = quantise(rng.standard_normal((experts * K, N)) / 8, dtype)
+    w[K, 0], w[2 * K - 1, N - 1] = np.inf, np.nan  # expert 1's first and last element
+    bad = np.zeros((rows, N), bool)
+    bad[0] = bad[experts + 2] = True
+    bad[ids[:, 0] == 1, 0] = bad[ids[:, 0] == 1, N - 1] = True
+    if act == 4:
+        bad = bad[:, :N // 2] | bad[:, N // 2:]
+    r = be.routing(rows, experts, 1)
+    r.assign(ids)
+    y = r.linear(tensor(fl, be, x[order] if grouped_input else x, dtype), tensor(fl, be, w, dtype), None, act, grouped_input).to_host()
+    seen = ~np.isfinite(y)
+    assert not (seen & ~bad[order]).any()
+    must = bad.copy()  # silu(-inf) and 0 * inf aside, what is not finite shows
+    if act == 4:
+        must[experts + 2] = False
+        must[ids[:, 0] == 1, 0] = False
+    assert seen[must[order]].all()
