@@ -177,7 +177,7 @@ __global__ void __launch_bounds__((BM / TM) * (BN / TN) * KS) k_grouped_simt(con
       float v = acc[0][i][j] + (bias ? to_f<T>(bias[n]) : 0.f);
       if constexpr (GATED) {
         const float u = acc[NB - 1][i][j] + (bias ? to_f<T>(bias[a.n_out + n]) : 0.f);
-        v = sizeof(T) == 4 ? swiglu_exact(v, u) : __fdividef(v, 1.0f + __expf(-v)) * u;
+        v = sizeof(T) == 4 ? swiglu_exact(v, u) : a.out32 ? swiglu_f32(v, u) : swiglu_16(v, u);
       } else {
         v = act1<T, ACT>(v);
       }

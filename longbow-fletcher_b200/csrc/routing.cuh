@@ -66,6 +66,10 @@ struct GroupedArgs {
   int32_t act;
   bool out32;  // 16-bit operands, fp32 result
 };
+// silu(g) * u of 16-bit operands.  An fp32 result takes expf and a division (under 5 half places off); one that is
+// rounded to 16 bits the special-function unit's, up to 30 half places of fp32 off.
+__device__ __forceinline__ float swiglu_f32(float g, float u) { return __fdiv_rn(g, 1.0f + expf(-g)) * u; }
+__device__ __forceinline__ float swiglu_16(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 bool grouped_tc_supported(int32_t dtype, const GroupedArgs& a);
 int64_t grouped_tc_workspace(const GroupedArgs& a);  // bytes
 int32_t launch_grouped_tc(Ctx* c, int32_t dtype, const GroupedArgs& a, void* workspace);

@@ -201,3 +201,24 @@ def test_nonfinite_row_stays_alone(fl, be, rows, experts, K, N, act, dtype, grou
         must[experts + 2] = False
         must[ids[:, 0] == 1, 0] = False
     assert seen[must[order]].all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,experts,k,K,half", [(2, 8, 2, 64, 64), (40, 4, 2, 64, 72), (300, 4, 1, 64, 72), (1000, 32, 2, 72, 520),
+                                                   (2100, 3, 1, 64, 776), (300, 3, 1, 65, 66)])
+def test_f32_swiglu_of_16_bit_operands(fl, be, rows, experts, k, K, half, dtype):  # noqa: F811
+    """An fp32 result is fp32 through the activation.  Each row picks one row of weights, so that gate and up
+    are exact; what is off is expf (2 u), an addition, a division and a product (u each)."""
+    rng = np.random.default_rng(rows + K)
+    ids = np.argsort(rng.random((rows, experts)), 1)[:, :k].astype(np.int32)
+    x = np.zeros((rows, K), np.float32)
+    x[np.arange(rows), np.arange(rows) % K] = 1.0
+    w = np.concatenate([quantise(rng.uniform(-30, 10, (experts * K, half)), dtype), quantise(rng.uniform(1, 2, (experts * K, half)), dtype)], 1)
+    r = be.routing(rows, experts, k)
+    r.assign(ids)
+    got = r.linear(tensor(fl, be, x, dtype), tensor(fl, be, w, dtype), None, fl.ACT_SWIGLU, dtype=fl.F32).to_host()
+    order = group_ref(ids, experts)[2]
+    picked = w[ids.reshape(-1)[order] * K + (order // k) % K].astype(np.float64)
+    want = picked[:, :half] / (1.0 + np.exp(-picked[:, :half])) * picked[:, half:]
+    off = np.abs(got - want) / np.maximum(np.abs(want), 1e-30)
+    assert off.max() <= 5 * E24 * (1 + 1e-5), off.max() / E24
