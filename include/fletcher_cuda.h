@@ -322,7 +322,8 @@ enum { FLETCHER_NORM_NONE = 0, FLETCHER_NORM_LAYER = 1, FLETCHER_NORM_RMS = 2 };
  * post and pre: none, LayerNorm ((x - mean) / sqrt(var + eps) * gamma + beta, as Cuda_LayerNorm)
  * or RMS (x / sqrt(mean(x^2) + eps) * gamma).  gamma and beta are f32 [cols]; NULL means 1 and 0;
  * RMS takes no beta.  residual [rows, cols] may be NULL (0).  gate may be NULL (1), or hold
- * gate_rows = 1 row for all or gate_rows = rows. */
+ * gate_rows = 1 row for all, or a row each: gate_rows >= rows, those behind not read (a buffer that is
+ * taller than this call's rows will do, as for every other input). */
 typedef struct FletcherBlockNorm {
   int32_t post_kind, pre_kind; /* FLETCHER_NORM_* */
   float eps;
@@ -335,14 +336,14 @@ typedef struct FletcherBlockNorm {
 } FletcherBlockNorm;
 /* u and h of y [rows, cols].  outResidual (u) may be NULL; outNorm (h) is given if and only if
  * pre_kind is not NONE.  Each output may be the same buffer as y, as the residual or as a gate of
- * `rows` rows.  cols <= 49152. */
+ * a row each.  cols <= 49152. */
 int32_t Cuda_BlockNorm(CudaContextRef ctx, CudaBufferRef y, int64_t rows, int64_t cols,
                        const FletcherBlockNorm* norm, CudaBufferRef outResidual, CudaBufferRef outNorm);
 /* Joins the experts' outputs (grouped [rows*top_k, cols], its slots as Cuda_Linear_Grouped wrote them,
  * in the other buffers' dtype or f32):
  *   y[r] = sum over the row's choices that have a slot, in order, of weight * grouped[slot]
  * in fp32, followed by Cuda_BlockNorm's u and h of y; norm NULL means u = y.  An output may be the
- * same buffer as the residual or as a gate of `rows` rows, not as `grouped`. */
+ * same buffer as the residual or as a gate of a row each, not as `grouped`. */
 int32_t Cuda_Combine_Grouped(CudaRoutingRef routing, CudaBufferRef grouped, int64_t cols,
                              const FletcherBlockNorm* norm, CudaBufferRef outResidual, CudaBufferRef outNorm);
 

@@ -31,10 +31,10 @@ int32_t setup(Ctx* c, const char* op, const Buf* y, int64_t y_rows, bool combine
   const Buf *res = reinterpret_cast<const Buf*>(n->residual), *gate = reinterpret_cast<const Buf*>(n->gate);
   FL_CHECK(c, !res || (res->dtype == dt && holds(c, res, total)), "%s: residual must be %lldx%lld of the input's dtype",
            op, (long long)rows, (long long)cols);
-  FL_CHECK(c, !gate || n->gate_rows == 1 || n->gate_rows == rows, "%s: gate_rows must be 1 or the rows", op);
-  const bool wide_gate = gate && n->gate_rows == rows && rows != 1;
+  FL_CHECK(c, !gate || n->gate_rows == 1 || n->gate_rows >= rows, "%s: gate_rows must be 1 or at least the rows", op);
+  const bool wide_gate = gate && n->gate_rows != 1 && rows != 1;
   FL_CHECK(c, !gate || (gate->dtype == dt && holds(c, gate, (wide_gate ? rows : 1) * cols)),
-           "%s: gate must be %lldx%lld of the input's dtype", op, (long long)n->gate_rows, (long long)cols);
+           "%s: gate must be %lldx%lld of the input's dtype", op, (long long)(wide_gate ? rows : 1), (long long)cols);
   const struct {
     CudaBufferRef ref;
     const float** to;
@@ -54,7 +54,7 @@ int32_t setup(Ctx* c, const char* op, const Buf* y, int64_t y_rows, bool combine
              "%s: an output overlaps the input", op);
     FL_CHECK(c, !res || o->ptr == res->ptr || !overlap(o->ptr, bytes, res->ptr, bytes),
              "%s: an output overlaps the residual", op);
-    FL_CHECK(c, !gate || (o->ptr == gate->ptr && n->gate_rows == rows) ||
+    FL_CHECK(c, !gate || (o->ptr == gate->ptr && (wide_gate || rows == 1)) ||
                     !overlap(o->ptr, bytes, gate->ptr, (wide_gate ? rows : 1) * cols * es),
              "%s: an output overlaps the gate", op);
   }

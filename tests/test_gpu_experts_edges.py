@@ -222,3 +222,20 @@ def test_f32_swiglu_of_16_bit_operands(fl, be, rows, experts, k, K, half, dtype)
     want = picked[:, :half] / (1.0 + np.exp(-picked[:, :half])) * picked[:, half:]
     off = np.abs(got - want) / np.maximum(np.abs(want), 1e-30)
     assert off.max() <= 5 * E24 * (1 + 1e-5), off.max() / E24
+
+
+@pytest.mark.parametrize("rows", [0, 1, 5])
+def test_taller_gate(fl, be, rows):  # noqa: F811
+    """A gate with more rows than the call has serves like a residual with more rows, in place too."""
+    rng = np.random.default_rng(rows)
+    y, gate = (rng.standard_normal((n, 24)).astype(np.float32) for n in (rows, 9))
+    ty, tg = tensor(fl, be, y, "f32"), tensor(fl, be, gate, "f32")
+    got, _ = ty.block_norm(fl.BlockNorm(gate=tg))
+    assert (got.to_host() == y * gate[:rows]).all()
+    r = be.routing(9, 2, 1)
+    r.assign(np.zeros((rows, 1)))
+    got, _ = r.combine(ty, fl.BlockNorm(gate=tg))
+    assert (got.to_host() == y * gate[:rows]).all()
+    ty.block_norm(fl.BlockNorm(gate=tg), out=tg)
+    assert (tg.to_host() == np.concatenate([y * gate[:rows], gate[rows:]])).all()
+    refuses(fl, be, lambda: tensor(fl, be, np.ones((10, 24)), "f32").block_norm(fl.BlockNorm(gate=tg)), "gate_rows")
