@@ -411,7 +411,7 @@ class Tensor:
         may be given (this tensor and the residual among them); with neither, u is made, and h if
         there is a pre norm.  A tensor that is neither given nor made is None."""
         out, out_norm = norm._outputs(self, self.rows, out, out_norm)
-        self.be.check(lib().Cuda_BlockNorm(self.be.ctx, self.buf, self.rows, self.cols, norm._ref(self.rows),
+        self.be.check(lib().Cuda_BlockNorm(self.be.ctx, self.buf, self.rows, self.cols, norm._ref(self.rows, self.cols),
                                            out.buf if out else None, out_norm.buf if out_norm else None))
         return out, out_norm
 
@@ -420,6 +420,12 @@ class Tensor:
         out = Tensor(self.be, lens.size, self.cols, F32)
         self.be.check(lib().Cuda_MeanPoolL2(self.be.ctx, self.buf, _i32p(lens), lens.size, self.cols, out.buf))
         return out
+
+
+def _dense(t, cols, what):
+    """Refuses a tensor whose rows are not `cols` wide; a flat one (one row or one column) holds them dense."""
+    if t is not None and t.cols != cols and t.rows != 1 and t.cols != 1:
+        raise FletcherError(1, f"{what} rows of {cols} columns, not {t.cols}")
 
 
 class CBlockNorm(ctypes.Structure):
@@ -442,13 +448,19 @@ class BlockNorm:
                             **{k: t.buf for k, t in self._tensors.items() if t is not None})
         self._p = ctypes.byref(self.c)
         self._residual_rows = residual.rows if residual is not None else float("inf")
+        self._cols = [(n, t.cols) for n, t in (("residual", residual), ("gate", gate)) if hasattr(t, "cols")]
 
-    def _ref(self, rows):
+    def _ref(self, rows, cols=None):
         if self._residual_rows < rows:
             raise FletcherError(1, f"BlockNorm: the residual has {self._residual_rows} rows, {rows} are needed")
+        for name, c in self._cols:
+            if c != cols and cols is not None:
+                raise FletcherError(1, f"BlockNorm: {name} must be of {cols} columns, not {c}")
         return self._p
 
     def _outputs(self, y, rows, out, out_norm, combine=False):
+        _dense(out, y.cols, "BlockNorm: outputs must be")
+        _dense(out_norm, y.cols, "BlockNorm: outputs must be")
         if out is None and out_norm is None:
             like = (self._tensors["residual"] or self._tensors["gate"] or y) if combine else y
             out = Tensor(y.be, rows, y.cols, like.dtype)
@@ -509,8 +521,11 @@ class Routing:
         x holds one row a token, or with grouped_input one row a slot.  The result has x's dtype, or F32."""
         if w.rows != self.num_experts * x.cols:
             raise FletcherError(1, f"Linear_Grouped: weight has {w.rows} rows, not {self.num_experts} x {x.cols}")
-        y = out or Tensor(self.be, self.rows * self.top_k, w.cols // 2 if act == ACT_SWIGLU else w.cols,
-                          x.dtype if dtype is None else dtype)
+        cols = w.cols // 2 if act == ACT_SWIGLU else w.cols
+        if act != ACT_SWIGLU or w.cols % 2 == 0:
+            _dense(out, cols, "Linear_Grouped: result must hold")
+        _dense(b, w.cols, "Linear_Grouped: bias must hold")
+        y = out or Tensor(self.be, self.rows * self.top_k, cols, x.dtype if dtype is None else dtype)
         self.be.check(lib().Cuda_Linear_Grouped(self.h, x.buf, ROWS_SLOTS if grouped_input else ROWS_TOKENS, x.cols,
                                                 w.buf, w.cols, b.buf if b is not None else None, y.buf, act))
         return y
@@ -520,11 +535,12 @@ class Routing:
         Without a norm returns the sum, else (u, h) as Tensor.block_norm does; tensors that are made have
         the residual's dtype, else the gate's, else grouped's."""
         if norm is None:
+            _dense(out, grouped.cols, "Combine_Grouped: outputs must be")
             out = out or Tensor(self.be, self.rows, grouped.cols, grouped.dtype)
             self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, None, out.buf, None))
             return out
         out, out_norm = norm._outputs(grouped, self.rows, out, out_norm, combine=True)
-        self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, norm._ref(self.rows),
+        self.be.check(lib().Cuda_Combine_Grouped(self.h, grouped.buf, grouped.cols, norm._ref(self.rows, grouped.cols),
                                                  out.buf if out else None, out_norm.buf if out_norm else None))
         return out, out_norm
 

@@ -239,3 +239,23 @@ def test_taller_gate(fl, be, rows):  # noqa: F811
     ty.block_norm(fl.BlockNorm(gate=tg), out=tg)
     assert (tg.to_host() == np.concatenate([y * gate[:rows], gate[rows:]])).all()
     refuses(fl, be, lambda: tensor(fl, be, np.ones((10, 24)), "f32").block_norm(fl.BlockNorm(gate=tg)), "gate_rows")
+
+
+def test_other_widths_are_refused(fl, be):  # noqa: F811
+    """A tensor that is large enough, but whose rows have another width, is not read or written at the wrong stride."""
+    new = lambda r, c: be.new_tensor(r, c, None, fl.BF16)  # noqa: E731
+    r = be.routing(8, 4, 2)
+    r.route(new(8, 4))
+    x, w, g = new(8, 16), new(64, 32), new(16, 32)
+    refuses(fl, be, lambda: r.linear(x, w, out=new(16, 40)), "result must hold")
+    refuses(fl, be, lambda: r.linear(x, w, None, fl.ACT_SWIGLU, out=new(16, 32)), "result must hold")
+    refuses(fl, be, lambda: r.linear(x, w, new(4, 40)), "bias must hold")
+    refuses(fl, be, lambda: r.combine(g, out=new(8, 40)), "outputs must be")
+    for kw, text in ((dict(residual=new(8, 40)), "residual must be"), (dict(gate=new(8, 40)), "gate must be"), (dict(gate=new(1, 40)), "gate must be")):
+        refuses(fl, be, lambda: r.combine(g, fl.BlockNorm(**kw)), text)
+        refuses(fl, be, lambda: new(8, 32).block_norm(fl.BlockNorm(**kw)), text)
+    refuses(fl, be, lambda: new(8, 32).block_norm(fl.BlockNorm(), out=new(8, 40)), "outputs must be")
+    refuses(fl, be, lambda: new(8, 32).block_norm(fl.BlockNorm(pre=1), out_norm=new(8, 40)), "outputs must be")
+    assert r.linear(x, w, new(1, 4 * 32), out=new(1, 16 * 32)).dims() == (1, 512)  # flat buffers hold the same rows
+    r.combine(g, out=new(1, 8 * 32))
+    be.synchronize()
