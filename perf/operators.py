@@ -161,6 +161,15 @@ def _logits(c, g, skew):
 
 
 def prepare(c, seed):
+    if own:
+        _fletcher()  # from here on its stream is torch's
+    s = _inputs(c, seed)
+    if own:
+        s["handles"] = _handles(s)
+    return s
+
+
+def _inputs(c, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     t = DTYPES[c["dtype"]]
 
@@ -335,6 +344,11 @@ def _fletcher():
     import fletcher
     if _backend is None:
         _backend = fletcher.Backend(0)
+        # The program works on the framework's stream: what torch computes before a call and after it is ordered
+        # with it, and nothing waits for that.
+        stream = torch.cuda.ExternalStream(_backend.stream())
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
     return fletcher, _backend
 
 
@@ -347,7 +361,9 @@ class _DeviceArray:
 
 
 def _handles(s):
-    """What a program keeps beside its buffers: their framework tensors, and the routing."""
+    """What a program keeps beside its buffers: their framework tensors, and the routing.  In the grouped and the
+    combine cases the routing was made before, by a router or by the program's own choice (a language's adapter),
+    and serves every product until the next one: it is the plan of these ids and weights, and the tensors stay."""
     fl, be = _fletcher()
     c = s["case"]
     dt = CODES[c["dtype"]]
@@ -390,7 +406,7 @@ def _handles(s):
 
 def _own(s):
     h = s.get("handles")
-    if h is None:
+    if h is None:  # a state of the plain form
         h = s["handles"] = _handles(s)
     c = s["case"]
     op = c["op"]
@@ -465,7 +481,7 @@ def _exact_norm(u, kind, gamma, beta):
 
 
 def exact(c, seed):
-    s = prepare(c, seed)
+    s = _inputs(c, seed)
     if c["op"] == "route":
         _, w = _exact_route(s["logits"], c["k"], c["score"], c["normalise"])
         return None, w, None, None
