@@ -496,32 +496,34 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSM) k_group(const RouteArg
 template <typename T, int L, int KM>
 int32_t route_l(Ctx* c, const RouteArgs& a, int blocks, bool one) {
   const size_t smem = (size_t)kWarps * a.E * 4;  // at most 16 KB
-  if (one) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = blocks;
-    at[1].val.clusterDim.y = 1;
-    at[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem + kSub * 2;
-    cfg.stream = c->stream;
-    cfg.attrs = at;
-    cfg.numAttrs = blocks > 1 ? 2 : 1;
-    FL_CUDA(c, cudaLaunchKernelEx(&cfg, k_route<T, L, KM, true>, a));
-    FL_LAUNCH(c);
-    return FLETCHER_OK;
+  if constexpr (L < 32) {  // a warp a row: few rows, which one cluster always holds
+    if (!one) {
+      FL_CUDA(c, launch_pdl(k_route<T, L, KM, false>, dim3(blocks), dim3(kThreads), 0, c->stream, a));
+      FL_LAUNCH(c);
+      const cudaError_t e = launch_pdl(k_group, dim3(blocks), dim3(kThreads), smem, c->stream, a);
+      if (e != cudaSuccess) {  // nobody clears the runs' counts
+        cudaMemsetAsync(a.spans, 0, (size_t)((blocks + kSpan - 1) / kSpan) * a.E * 4, c->stream);
+        FL_CUDA(c, e);
+      }
+      FL_LAUNCH(c);
+      return FLETCHER_OK;
+    }
   }
-  FL_CUDA(c, launch_pdl(k_route<T, L, KM, false>, dim3(blocks), dim3(kThreads), 0, c->stream, a));
-  FL_LAUNCH(c);
-  const cudaError_t e = launch_pdl(k_group, dim3(blocks), dim3(kThreads), smem, c->stream, a);
-  if (e != cudaSuccess) {  // nobody clears the runs' counts
-    cudaMemsetAsync(a.spans, 0, (size_t)((blocks + kSpan - 1) / kSpan) * a.E * 4, c->stream);
-    FL_CUDA(c, e);
-  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = blocks;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem + kSub * 2;
+  cfg.stream = c->stream;
+  cfg.attrs = at;
+  cfg.numAttrs = blocks > 1 ? 2 : 1;
+  FL_CUDA(c, cudaLaunchKernelEx(&cfg, k_route<T, L, KM, true>, a));
   FL_LAUNCH(c);
   return FLETCHER_OK;
 }
@@ -529,13 +531,18 @@ int32_t route_l(Ctx* c, const RouteArgs& a, int blocks, bool one) {
 template <typename T, int L>
 int32_t route_k(Ctx* c, const RouteArgs& a, int blocks, bool one) {
   if (a.k <= 2) return route_l<T, L, 2>(c, a, blocks, one);
-  if (a.k <= 8) return route_l<T, L, 8>(c, a, blocks, one);
-  return route_l<T, L, 16>(c, a, blocks, one);
+  if constexpr (L > 1)  // one lane: at most 8 experts
+    if (a.k > 8) return route_l<T, L, 16>(c, a, blocks, one);
+  return route_l<T, L, 8>(c, a, blocks, one);
 }
 
 // Lanes a row: one where a chunk holds all experts; a warp for few rows of many experts, where the chain of
 // chunks is what takes time (128 x 256 -> 8: 6.1 us, 9.6 with four; 32 x 64 -> 6: 5.3 against 4.2).
-int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E > 8 * V && a.rows <= 128 ? 32 : 4; }
+constexpr int kWarpRowsMost = 128;
+static_assert((kWarpRowsMost + kSub / kMaxTopK - 1) / (kSub / kMaxTopK) <= kClusterMost &&
+                  (kWarpRowsMost + kWarps - 1) / kWarps <= 2 * kClusterMost,
+              "one launch takes as many rows, whatever top_k");
+int lanes_of(const RouteArgs& a) { return a.E <= V ? 1 : a.E > 8 * V && a.rows <= kWarpRowsMost ? 32 : 4; }
 
 template <typename T>
 int32_t route_t(Ctx* c, const RouteArgs& a, int blocks, bool one) {

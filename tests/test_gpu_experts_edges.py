@@ -259,3 +259,19 @@ def test_other_widths_are_refused(fl, be):  # noqa: F811
     assert r.linear(x, w, new(1, 4 * 32), out=new(1, 16 * 32)).dims() == (1, 512)  # flat buffers hold the same rows
     r.combine(g, out=new(1, 8 * 32))
     be.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [127, 128, 129])
+@pytest.mark.parametrize("experts,k", [(64, 16), (65, 1), (256, 16), (200, 9), (8, 8), (8, 3), (9, 9)])
+def test_routing_between_lane_counts(fl, be, rows, experts, k, dtype):  # noqa: F811
+    """One, four and 32 lanes a row, on both sides of where they change."""
+    rng = np.random.default_rng(rows + experts)
+    z = quantise(np.round(8 * rng.standard_normal((rows, experts))) / 4, dtype)
+    r = be.routing(rows, experts, k)
+    r.route(tensor(fl, be, z, dtype))
+    got = r.read()
+    ids, w = route_ref(z, k)
+    slots, offsets, _ = group_ref(ids, experts)
+    assert (got["experts"] == ids).all() and (got["slots"] == slots).all() and (got["offsets"] == offsets).all()
+    assert np.allclose(got["weights"], w, rtol=64 * E24, atol=0)
