@@ -255,10 +255,11 @@ int32_t Cuda_MeanPoolL2(CudaContextRef ctx, CudaBufferRef hidden, const int32_t*
  *     device alone and never wait for the GPU, so that a sequence of them can be captured into a
  *     CUDA graph (except Cuda_Routing_Create, Assign and Read, which allocate or use host arrays: during a
  *     capture they fail and leave it as it was);
- *   - Cuda_Linear_Grouped of token rows keeps a workspace with its routing (up to rows * top_k *
- *     inCols elements, at most doubled), which a call that needs more makes larger; earlier ones
- *     stay valid until the routing is freed.  During a capture it cannot grow: the call fails, so
- *     make it once before;
+ *   - Cuda_Linear_Grouped of token rows keeps a workspace with its routing: rows * top_k * inCols
+ *     elements, or twice the last one where a call outgrows that (where twice cannot be had, just what the call
+ *     needs).  Earlier ones stay valid until the routing is freed, as captured graphs may use them; all
+ *     together are less than four times the largest need, and exactly that need where the largest call
+ *     came first.  During a capture it cannot grow: the call fails, so make it once before;
  *   - buffers are dense and row-major, and share one dtype except where noted;
  *   - an output may not overlap an input unless its entry below says so.
  *

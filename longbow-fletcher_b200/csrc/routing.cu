@@ -606,7 +606,8 @@ int32_t routing_workspace(Routing* r, int64_t bytes, void** out) {
     FL_CHECK(c, st == cudaStreamCaptureStatusNone,
              "Linear_Grouped: the routing's workspace must grow; make the call once before capturing it");
     FL_CHECK(c, n < Routing::kMaxBlocks, "Linear_Grouped: the routing's workspace cannot grow further");
-    // Twice the last block: what was outgrown adds up to less than the newest.
+    // Twice the last block: what was outgrown adds up to less than the newest, and that is less than twice the
+    // largest need.
     const int64_t want = std::max(bytes, n ? 2 * r->work_bytes[n - 1] : 0);
     int32_t rc = dev_alloc(c, &r->work[n], want);
     r->work_bytes[n] = want;

@@ -275,3 +275,20 @@ def test_routing_between_lane_counts(fl, be, rows, experts, k, dtype):  # noqa: 
     slots, offsets, _ = group_ref(ids, experts)
     assert (got["experts"] == ids).all() and (got["slots"] == slots).all() and (got["offsets"] == offsets).all()
     assert np.allclose(got["weights"], w, rtol=64 * E24, atol=0)
+
+
+def test_workspace_bound(fl, be):  # noqa: F811
+    """However the needs grow, a routing holds less than four times the largest; the largest first, just that."""
+    E, k, K, N = 2, 2, 256, 64
+    w = be.new_tensor(E * K, N, None, fl.BF16)
+    for needs, most in (((400, 404, 804, 1612), 4), ((1612, 400, 804), 1)):
+        r = be.routing(2000, E, k)
+        x, y = be.new_tensor(2000, K, None, fl.BF16), be.new_tensor(2000 * k, N, None, fl.BF16)
+        before = be.vram_usage()[0]
+        for rows in needs:
+            r.assign(np.tile([0, 1], (rows, 1)))
+            r.linear(x, w, out=y)
+        held = be.vram_usage()[0] - before
+        assert max(needs) * k * K * 2 <= held <= most * max(needs) * k * K * 2, held
+        be.synchronize()
+        del r, x, y
