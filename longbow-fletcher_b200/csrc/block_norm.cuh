@@ -236,16 +236,17 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
     s = -1;
     if (r < a.rows && lane < a.top_k) {
       s = a.slots[r * a.top_k + lane];
-      if (s >= a.num_slots) s = -1;
       f = a.weights[r * a.top_k + lane];
     }
   };
+  // Asked where a slot is used, not where it is loaded: that would wait for the load (32768 x 2 x 768: 41 us).
+  auto some = [&](int32_t s) { return (uint32_t)s < (uint32_t)a.num_slots; };
   auto load_y = [&](int64_t r, int32_t s) {
     if constexpr (COMBINE) {
 #pragma unroll
       for (int j = 0; j < NY; j++) {
         const int32_t sj = __shfl_sync(0xffffffffu, s, j);  // -1 past the choices
-        if (sj >= 0) load(py[j], a.y, sj);
+        if (some(sj)) load(py[j], a.y, sj);
       }
     } else if (r < a.rows) {
       load(py[0], a.y, r);
@@ -285,12 +286,12 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks<VEC, NV>) k_block_norm(co
 #pragma unroll
       for (int j = 0; j < NY; j++) {
         const float wj = __shfl_sync(0xffffffffu, w, j);
-        if (__shfl_sync(0xffffffffu, slot, j) >= 0) add(py[j], wj);
+        if (some(__shfl_sync(0xffffffffu, slot, j))) add(py[j], wj);
       }
       for (int j = NY; j < a.top_k; j++) {
         const int32_t sj = __shfl_sync(0xffffffffu, slot, j);
         const float wj = __shfl_sync(0xffffffffu, w, j);
-        if (sj >= 0) {
+        if (some(sj)) {
           load(py[0], a.y, sj);
           add(py[0], wj);
         }
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kThreads) k_block_norm_generic(const NormArgs 
       if constexpr (COMBINE) {
         for (int j = 0; j < a.top_k; j++) {
           const int32_t slot = a.slots[row * a.top_k + j];
-          if (slot >= 0 && slot < a.num_slots) s = fmaf(a.weights[row * a.top_k + j], to_f<TY>(y[(int64_t)slot * a.cols + c]), s);
+          if ((uint32_t)slot < (uint32_t)a.num_slots) s = fmaf(a.weights[row * a.top_k + j], to_f<TY>(y[(int64_t)slot * a.cols + c]), s);
         }
       } else {
         s = to_f<TY>(y[row * a.cols + c]);
