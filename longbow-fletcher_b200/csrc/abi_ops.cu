@@ -53,10 +53,11 @@ int32_t packed_weight(Ctx* c, Buf* w, int64_t K, int64_t N, bool swiglu, int bn,
     w->packed_bytes = bytes;
   }
   // A wrapped weight (the caller's memory) may have changed unseen: laid out in every call.
-  if (w->external || w->packed_key != key || w->packed_ver != w->version) {
+  if (w->external || w->packed_key != key || w->packed_k != K || w->packed_ver != w->version) {
     w->packed_key = -1;
     if ((rc = launch_pack_kmajor_16(c, w->dtype, w->ptr, K, N, w->packed, swiglu ? 1 : 0, bn))) return rc;
     w->packed_key = key;
+    w->packed_k = K;
     w->packed_ver = w->version;
   }
   *out = w->packed;

@@ -45,14 +45,15 @@ struct Buf {
   int64_t rows = 0, cols = 0;
   int32_t dtype = FLETCHER_F32;
   int device = 0;         // where the memory is
-  bool external = false;  // the caller's memory (Cuda_WrapTensor): never freed, nothing derived is kept
+  bool external = false;  // the caller's memory (Cuda_WrapTensor): never freed, what is derived from it is made anew in every call
   // Write counter: bumped by every ABI call that may change the contents (see touch()).
   uint64_t version = 0;
   // Cuda_Linear_Fused's derived copies of a 16-bit weight / bias, valid while `version` equals
-  // the recorded one and the layout key (SwiGLU interleave, tile width) matches.
+  // the recorded one and the layout key (SwiGLU interleave, tile width) and the weight's rows match.
   void* packed = nullptr;
   int64_t packed_bytes = 0;
   int packed_key = -1;
+  int64_t packed_k = 0;
   uint64_t packed_ver = 0;
   float* bias32 = nullptr;
   int64_t bias32_bytes = 0;

@@ -292,3 +292,19 @@ def test_workspace_bound(fl, be):  # noqa: F811
         assert max(needs) * k * K * 2 <= held <= most * max(needs) * k * K * 2, held
         be.synchronize()
         del r, x, y
+
+
+def test_weight_read_in_two_shapes(fl, be):  # noqa: F811
+    """One weight buffer as (256, 512) and then as (512, 256): the same bytes, but not the same layout."""
+    rng = np.random.default_rng(6)
+    w = quantise(rng.standard_normal(256 * 512) / 16, "bf16")
+    tw = tensor(fl, be, w.reshape(256, 512), "bf16")
+    for K in (256, 512, 256):
+        x = quantise(rng.standard_normal((40, K)), "bf16")
+        N = w.size // K
+        ty = be.new_tensor(40, N, None, fl.BF16)
+        tx = tensor(fl, be, x, "bf16")  # kept: the call takes its handle
+        be.check(fl.lib().Cuda_Linear_Fused(be.ctx, tx.buf, 40, K, tw.buf, N, None, ty.buf, 0))
+        want = x.astype(np.float64) @ w.reshape(K, N)
+        mag = np.abs(x.astype(np.float64)) @ np.abs(w.reshape(K, N))
+        assert (np.abs(ty.to_host() - want) <= np.abs(want) * U["bf16"] * 1.01 + (K + 4) * E24 * mag).all()
