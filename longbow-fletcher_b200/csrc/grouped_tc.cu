@@ -174,16 +174,12 @@ __device__ __forceinline__ void gelu_pair(float& x0, float& x1) {
   fma2(x0, x1, x0, x1, t0, t1, x0, x1);
 }
 
-// A lane's 32 gates and ups.  The choice stands outside the loops: with it inside, 32768 x 2 rows of 8 experts,
-// 768 -> 2 x 2048, took 484 us against 384.
-__device__ __forceinline__ void swiglu32(bool f32, const float (&g)[32], const float (&u)[32], float* v) {
-  if (f32) {
+// A lane's 32 gates and ups; F32: for an fp32 result.  (Chosen at run time, the form that is not taken cost the
+// large product 1.5%: 292 against 287.5 us at 32768 x 2 rows of 8 experts, 768 -> 2 x 2048.)
+template <bool F32>
+__device__ __forceinline__ void swiglu32(const float (&g)[32], const float (&u)[32], float* v) {
 #pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = swiglu_f32(g[i], u[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = swiglu_16(g[i], u[i]);
-  }
+  for (int i = 0; i < 32; i++) v[i] = F32 ? swiglu_f32(g[i], u[i]) : swiglu_16(g[i], u[i]);
 }
 
 __device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
@@ -216,7 +212,7 @@ __device__ __forceinline__ void store_row(const Args& args, const float* v, int6
 // Persistent: warp 0 loads by TMA, warp 1 issues the MMAs and owns the TMEM, warps 2-9 drain one
 // accumulator while the next tile fills the other.  As the dense GEMM: bounded waits, and
 // on expiry every role leaves after what it issued has landed.
-template <typename T, int BN, bool PAIR, bool GATED>
+template <typename T, int BN, bool PAIR, bool GATED, bool F32>
 __global__ void __launch_bounds__(kThreads, 1)
     k_grouped_tc(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const Args args) {
@@ -414,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               add_bias32<T>(g, bias, ocol + s * 32, args.n_out);
               add_bias32<T>(w, bias + args.n_out, ocol + s * 32, args.n_out);
             }
-            swiglu32(args.out32, g, w, &v[s * 32]);
+            swiglu32<F32>(g, w, &v[s * 32]);
           }
         } else {
           tmem_ld32x2(tbase + c0, lo, hi);
@@ -504,7 +500,7 @@ __device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-template <typename T, bool GATED, bool GATHER, bool SPLIT>
+template <typename T, bool GATED, bool GATHER, bool SPLIT, bool F32>
 __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
     k_grouped_small(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Args args) {
   using C = SmallCfg;
@@ -651,7 +647,7 @@ __global__ void __launch_bounds__(SmallCfg::kThreads, 1)
         add_bias32<T>(hi, bias, ocol + 32, args.n_out);
     }
     if constexpr (GATED) {
-      swiglu32(args.out32, lo, hi, v);
+      swiglu32<F32>(lo, hi, v);
     } else if (args.act == FLETCHER_ACT_GELU) {
 #pragma unroll
       for (int i = 0; i < 64; i += 2) gelu_pair(v[i], v[i + 1]);
@@ -754,7 +750,7 @@ int64_t most_tiles(const GroupedArgs& g, int tile_m, int n_tiles) {
   return (g.pairs / tile_m + std::min<int64_t>(g.experts, g.pairs)) * n_tiles;
 }
 
-template <typename T, bool GATED, bool GATHER, bool SPLIT>
+template <typename T, bool GATED, bool GATHER, bool SPLIT, bool F32>
 int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g, int ranks) {
   using C = SmallCfg;
   CUtensorMap ma, mb;
@@ -764,7 +760,7 @@ int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g, int ranks) {
     return rc;
   if ((rc = make_tma_map_3d(c, &mb, dt, g.w, (uint64_t)g.experts, (uint64_t)g.K, (uint64_t)g.N, 64, BK))) return rc;
   const Args a = args_of(c, g, GATED ? C::BN / 2 : C::BN);
-  auto kern = k_grouped_small<T, GATED, GATHER, SPLIT>;
+  auto kern = k_grouped_small<T, GATED, GATHER, SPLIT, F32>;
   static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
   if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
     FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
@@ -790,25 +786,29 @@ int32_t run_small(Ctx* c, int32_t dt, const GroupedArgs& g, int ranks) {
   return FLETCHER_OK;
 }
 
-template <typename T, bool GATED, bool GATHER>
+template <typename T, bool GATED, bool GATHER, bool F32>
 int32_t launch_small_g(Ctx* c, int32_t dt, const GroupedArgs& g) {
   // CTAs a tile: as many as the SMs have room for, at most 8, two slabs of K each at least.
   const int out_n = GATED ? SmallCfg::BN / 2 : SmallCfg::BN;
   const int64_t tiles = most_tiles(g, SmallCfg::TILE_M, (int)((g.n_out + out_n - 1) / out_n));
   int ranks = 1;
   while (ranks < 8 && tiles * ranks * 2 <= c->num_sms && g.K >= ranks * 4 * BK) ranks *= 2;
-  return ranks > 1 ? run_small<T, GATED, GATHER, true>(c, dt, g, ranks) : run_small<T, GATED, GATHER, false>(c, dt, g, 1);
+  return ranks > 1 ? run_small<T, GATED, GATHER, true, F32>(c, dt, g, ranks)
+                   : run_small<T, GATED, GATHER, false, F32>(c, dt, g, 1);
+}
+
+template <typename T, bool GATHER>
+int32_t launch_small_a(Ctx* c, int32_t dt, const GroupedArgs& g) {
+  if (g.act != FLETCHER_ACT_SWIGLU) return launch_small_g<T, false, GATHER, false>(c, dt, g);
+  return g.out32 ? launch_small_g<T, true, GATHER, true>(c, dt, g) : launch_small_g<T, true, GATHER, false>(c, dt, g);
 }
 
 template <typename T>
 int32_t launch_small(Ctx* c, int32_t dt, const GroupedArgs& g) {
-  const bool gather = g.pair_of != nullptr;
-  if (g.act == FLETCHER_ACT_SWIGLU)
-    return gather ? launch_small_g<T, true, true>(c, dt, g) : launch_small_g<T, true, false>(c, dt, g);
-  return gather ? launch_small_g<T, false, true>(c, dt, g) : launch_small_g<T, false, false>(c, dt, g);
+  return g.pair_of ? launch_small_a<T, true>(c, dt, g) : launch_small_a<T, false>(c, dt, g);
 }
 
-template <typename T, int BN, bool PAIR, bool GATED>
+template <typename T, int BN, bool PAIR, bool GATED, bool F32>
 int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
   using C = Cfg<BN, PAIR>;
   constexpr int OUT_N = GATED ? BN / 2 : BN;
@@ -822,7 +822,7 @@ int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
       (rc = make_tma_map_2d(c, &mc, dt, g.out, (uint64_t)g.pairs, (uint64_t)g.n_out, (uint64_t)g.n_out, 64, 32)))
     return rc;
   const Args a = args_of(c, g, OUT_N);
-  auto kern = k_grouped_tc<T, BN, PAIR, GATED>;
+  auto kern = k_grouped_tc<T, BN, PAIR, GATED, F32>;
   static std::atomic<bool> attr_set[64] = {};  // per device; idempotent, replicas' threads may meet here
   if (!attr_set[c->device & 63].load(std::memory_order_acquire)) {
     FL_CUDA(c, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
@@ -851,7 +851,8 @@ int32_t run(Ctx* c, int32_t dt, const GroupedArgs& g) {
 
 template <typename T, int BN, bool PAIR>
 int32_t pick(Ctx* c, int32_t dt, const GroupedArgs& g) {
-  return g.act == FLETCHER_ACT_SWIGLU ? run<T, BN, PAIR, true>(c, dt, g) : run<T, BN, PAIR, false>(c, dt, g);
+  if (g.act != FLETCHER_ACT_SWIGLU) return run<T, BN, PAIR, false, false>(c, dt, g);
+  return g.out32 ? run<T, BN, PAIR, true, true>(c, dt, g) : run<T, BN, PAIR, true, false>(c, dt, g);
 }
 
 // Token rows copied to their slots: a warp a token, whose row is read once and written for each of its
