@@ -284,7 +284,7 @@ enum { FLETCHER_SCORE_SOFTMAX = 0, FLETCHER_SCORE_SIGMOID = 1 };
  * top_k largest logits in descending order, equal ones by the lower expert; -inf and NaN are never
  * chosen, and a row with fewer than top_k others gets -1 with weight 0 for the rest.  The weight of
  * a choice is the softmax over the row's eligible logits (if some are +inf they share the weight equally)
- * or the logit's sigmoid; with normalise != 0 the weights of a row are divided by
+ * or the logit's sigmoid (in fp32: 0 below about -88.7); with normalise != 0 the weights of a row are divided by
  * their sum (all 0 if that is 0); then all are multiplied by `scale`.  Weights are f32. */
 int32_t Cuda_Routing_TopK(CudaRoutingRef routing, CudaBufferRef logits, int64_t rows, int32_t scoring,
                           int32_t normalise, float scale);

@@ -52,9 +52,10 @@ __device__ __forceinline__ float act1(float v) {
 // One BM x BN output tile a block (SwiGLU: its gate and up columns), TM x TN sums a thread in packed pairs
 // along n, K in slabs of 16: the next slab's elements are on their way from memory while this one's are
 // multiplied from shared memory.  Rows are gathered as they are loaded; single elements, so that any
-// width does.  KS teams of threads take alternate slabs.  Bound by the fp32 units (34
-// TFLOP/s at 4000 x 2 rows of 8 experts, 500 -> 500), for few rows by a slab's chain of load, store and
-// multiply, which teams overlap.
+// width does.  KS teams of threads take alternate slabs.  At 4000 x 2 rows of 8
+// experts, 500 -> 500, it gives 34 TFLOP/s, under half of the fp32 units' rate (74 at 1.95 GHz): beside the packed
+// multiply-adds stand single loads with a test each, transposing stores and the (x, x) pairs.  Few rows are
+// bound by a slab's chain of load, store and multiply, which teams overlap.
 template <typename T, int ACT, int BM, int BN, int TM, int TN, int KS>
 __global__ void __launch_bounds__((BM / TM) * (BN / TN) * KS) k_grouped_simt(const GroupedArgs a) {
   constexpr int BK = 16, kThreads = (BM / TM) * (BN / TN);  // of one of the KS teams

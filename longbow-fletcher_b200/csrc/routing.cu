@@ -7,10 +7,11 @@
 // and merge it in; two choices are kept by insertion); then a round takes the largest of the lanes'
 // first keys (log2 L shuffles) and its owner moves on.  Lane j mod L keeps
 // choice j and computes its exponential, with the first winner as the maximum; exponentials and quotients
-// are those of full fp32 precision (the special-function unit's took 17.4 us where these take 18.5 and lost
-// up to 16 places where x - m is -30).  Bound by instruction issue for half of its time, else by latency of
-// loads and of the two launches: 65536 x 64 -> 6 in 18.5 us, 16.8 where only chosen weights are summed.  Four lanes
-// a row for many rows (two and eight were within 1 us there, at 16384 x 128 -> 8 slower by 5 and 1).
+// are expf's and a division's (with the special-function unit's exponential 17.4 us where these take 18.4, and
+// weights 30 below the maximum off by up to 14 units of their last place).  65536 x 64 -> 6: 18.4 us, 16.9 where only
+// the chosen weights are summed.  Issuing the two kernels' 11.1 M warp instructions takes half of that; the rest is
+// latency, of loads and of two dependent launches.  Four lanes a row for many rows (two and eight were within
+// 1 us there, at 16384 x 128 -> 8 slower by 5 and 1).
 //
 // Grouping is a stable counting sort in two launches: k_route leaves, per block of rows and per run of
 // kSpan blocks, how many choices each expert got; k_group sums the runs and blocks before its own, ranks
@@ -83,13 +84,13 @@ struct KeyOf<__half> : KeyOf16<__half, __half2, 0xfc00u> {};
 template <>
 struct KeyOf<__nv_bfloat16> : KeyOf16<__nv_bfloat16, __nv_bfloat162, 0xff80u> {};
 
-// Eight keys in descending order.
 template <typename K>
 __device__ __forceinline__ void exchange(K& a, K& b) {
   const K hi = a > b ? a : b, lo = a > b ? b : a;
   a = hi;
   b = lo;
 }
+// Eight keys in descending order, by Batcher's odd-even merge sort: 19 exchanges.
 template <typename K>
 __device__ __forceinline__ void sort8(K (&k)[8]) {
   auto ex = [&](int i, int j) { exchange(k[i], k[j]); };
@@ -537,7 +538,7 @@ int32_t route_k(Ctx* c, const RouteArgs& a, int blocks, bool one) {
 }
 
 // Lanes a row: one where a chunk holds all experts; a warp for few rows of many experts, where the chain of
-// chunks is what takes time (128 x 256 -> 8: 6.1 us, 9.6 with four; 32 x 64 -> 6: 5.3 against 4.2).
+// chunks is what takes time (128 x 256 -> 8: 5.8 us, 9.0 with four; 32 x 64 -> 6: 5.4 against 4.1).
 constexpr int kWarpRowsMost = 128;
 static_assert((kWarpRowsMost + kSub / kMaxTopK - 1) / (kSub / kMaxTopK) <= kClusterMost &&
                   (kWarpRowsMost + kWarps - 1) / kWarps <= 2 * kClusterMost,
@@ -570,7 +571,7 @@ int32_t route(Routing* r, int32_t dtype, RouteArgs a) {
   const int64_t pass = kThreads / lanes_of(a);  // rows a block takes at once
   const int64_t passes = std::max<int64_t>(1, (a.rows + pass - 1) / pass);
   // One launch where a cluster's blocks hold the pairs and take no more than two turns (4096 x 64 -> 6 in
-  // four turns: 15.9 us, in two launches 9.5; 4096 x 8 -> 2: 5.5 against 7.8).
+  // four turns: 15.4 us, in two launches 9.3; 4096 x 8 -> 2: 5.2 against 7.6).
   const int64_t fit = (a.rows + kSub / a.k - 1) / (kSub / a.k);  // blocks of at most kSub pairs
   const bool one = fit <= kClusterMost && passes <= 2 * kClusterMost;
   int64_t blocks = std::max(fit, std::min<int64_t>(passes, one ? kClusterMost : max_blocks(c)));
